@@ -306,6 +306,69 @@ typedef struct {
 } Dsv41ArgmaxArgs;
 int dsv41_argmax_decode(const Dsv41ArgmaxArgs* a, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit GEMV
+ * y[m][n] = sum_k x[m][k] * (w[n][k] - z[n][k / group]) * s[n][k / group], summed in fp32 and
+ * rounded once to x's type: w unsigned 4-bit values packed two a byte, [N, K / 2] row-major (even
+ * k in the low nibble) and read in place; scales [N, K / group] of x's type; zeros u8
+ * [N, K / group] (values 0 .. 15) or 0 for 8 everywhere; x [M, x_ld] and y [M, y_ld] bf16, or f16
+ * with f16 = 1. M <= 48, K a multiple of group, group a multiple of 32; w and x 16-byte aligned,
+ * x_ld a multiple of 8. No counterpart in the reference (its dense projections are FP8). */
+typedef struct {
+  int64_t w, scales, zeros, x, y;     /* device pointers */
+  int64_t M, N, K, group, x_ld, y_ld, f16;
+} Dsv41GemvW4Args;
+int dsv41_gemv_w4(const Dsv41GemvW4Args* a, void* stream);
+
+/* ---------------------------------------------------------------- Paged 8-bit KV cache
+ * Grouped-query keys and values in e4m3 with one E8M0 code per `block` consecutive tokens of a
+ * head: k_cache, v_cache [pages, kv_heads, page, dim] bytes, k_codes, v_codes
+ * [pages, kv_heads, page / block]. Sequence s holds lens[s] tokens (int32); its token p lies at
+ * page table[s][p / page] (int32 [seqs, width], rows table_ld apart), offset p % page. The rows of
+ * a step lie one sequence after the other: sequence s has rows cu_rows[s] .. cu_rows[s + 1] (int32
+ * [seqs + 1]), or row s alone with cu_rows = 0 (T = seqs); they are its last tokens, so row j of n
+ * is token lens[s] - n + j. Rows behind cu_rows[seqs] belong to no sequence: nothing is read or
+ * written for them. dim 64, 128 or 256; block a multiple of 16, page a multiple of block; rows
+ * [T, heads, dim] bf16 (f16 = 1: f16), a row's heads contiguous, rows *_ld elements apart (a
+ * multiple of 8), 16-byte aligned.
+ *
+ * dsv41_kv_append writes the rows' keys and values into the cache (lens counts them already), with
+ * the position rotation on the way: the last `rope` dims of every key turn by the angles of
+ * cos_sin [rope_rows, rope] fp32 (rope / 2 cos, then rope / 2 sin; a position past the table reads
+ * its last row) in pairs (2j, 2j + 1), or (j, j + rope / 2) with neox = 1, products and sums
+ * rounded separately in fp32; rope = 0: none. With q (optional) q_out gets the queries rotated the
+ * same way (q_out may be q). A block's code: the smallest power of two c with
+ * max(amax, 1e-4) / 448 <= c over its new tokens, and not below the code that its older tokens
+ * have; when it grows, the older tokens' bytes are rounded again to the new scale. Values are
+ * rounded to nearest even and saturate at 448 c; an infinity counts as the largest float, NaN stays
+ * NaN and moves no scale. Tokens whose page is out of range (table entry outside [0, pages), or a
+ * position outside [0, width * page)) are skipped. No counterpart in the reference (its records
+ * hold one shared latent a token with a scale per token, front.py:246-300). */
+typedef struct {
+  int64_t T, seqs, heads, kv_heads, dim, rope, neox, f16;
+  int64_t q, q_ld, q_out, q_out_ld, k, k_ld, v, v_ld, cos_sin, rope_rows;
+  int64_t cu_rows, lens, table, table_ld, width;
+  int64_t k_cache, v_cache, k_codes, v_codes, pages, page, block;
+} Dsv41KvAppendArgs;
+int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream);
+
+/* Attention of a step's rows over that cache: row j of n sees the keys before vis = lens[s] - n +
+ * j + 1, the last `window` of them with window > 0; out = sum_i softmax(scale q . k)_i v_i per
+ * head, heads / kv_heads query heads a kv head, softmax and sums in fp32; sink (fp32 [heads],
+ * optional) is one more score that has no value. A row that sees no key gives 0. Keys on pages out
+ * of range are not seen. scale_f32: the fp32 bit pattern. Decode and verify rows: few rows a
+ * sequence over a long cache. Replaces, for grouped-query heads, what back.py:189-435 of the
+ * reference does for its shared latent. */
+typedef struct {
+  int64_t T, seqs, heads, kv_heads, dim, f16;
+  int64_t q, q_ld, out, out_ld;
+  int64_t cu_rows, lens, table, table_ld, width;
+  int64_t k_cache, v_cache, k_codes, v_codes, pages, page, block;
+  int64_t scale_f32, window, sink;
+  int64_t scratch, scratch_bytes;
+} Dsv41PagedAttnArgs;
+int64_t dsv41_paged_attn_scratch_bytes(const Dsv41PagedAttnArgs* a);
+int dsv41_paged_attn(const Dsv41PagedAttnArgs* a, void* stream);
+
 /* DSV41_EDEVICE once a kernel's bounded internal wait gave up in this process (the tcgen05
  * attention's and the routed experts' pipeline barriers; sticky), else 0. Synchronizes with the device. */
 int dsv41_device_error(void);

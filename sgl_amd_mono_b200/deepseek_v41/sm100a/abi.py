@@ -80,6 +80,26 @@ LmHeadArgs = struct("Dsv41LmHeadArgs", ["M", "V", "K", "vbase", "w", "x", "logit
 
 ArgmaxArgs = struct("Dsv41ArgmaxArgs", ["M", "best", "ids", "vals", "draft", "per_req", "accept", "next_tok"])
 
+GemvW4Args = struct("Dsv41GemvW4Args", [
+    "w", "scales", "zeros", "x", "y", "M", "N", "K", "group", "x_ld", "y_ld", "f16",
+])
+
+KvAppendArgs = struct("Dsv41KvAppendArgs", [
+    "T", "seqs", "heads", "kv_heads", "dim", "rope", "neox", "f16",
+    "q", "q_ld", "q_out", "q_out_ld", "k", "k_ld", "v", "v_ld", "cos_sin", "rope_rows",
+    "cu_rows", "lens", "table", "table_ld", "width",
+    "k_cache", "v_cache", "k_codes", "v_codes", "pages", "page", "block",
+])
+
+PagedAttnArgs = struct("Dsv41PagedAttnArgs", [
+    "T", "seqs", "heads", "kv_heads", "dim", "f16",
+    "q", "q_ld", "out", "out_ld",
+    "cu_rows", "lens", "table", "table_ld", "width",
+    "k_cache", "v_cache", "k_codes", "v_codes", "pages", "page", "block",
+    "scale_f32", "window", "sink",
+    "scratch", "scratch_bytes",
+])
+
 STRUCTS = {
     "Dsv41GemvArgs": GemvArgs,
     "Dsv41RelayoutArgs": RelayoutArgs,
@@ -95,4 +115,7 @@ STRUCTS = {
     "Dsv41RankSumArgs": RankSumArgs,
     "Dsv41LmHeadArgs": LmHeadArgs,
     "Dsv41ArgmaxArgs": ArgmaxArgs,
+    "Dsv41GemvW4Args": GemvW4Args,
+    "Dsv41KvAppendArgs": KvAppendArgs,
+    "Dsv41PagedAttnArgs": PagedAttnArgs,
 }

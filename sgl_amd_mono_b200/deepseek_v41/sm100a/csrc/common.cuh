@@ -292,4 +292,7 @@ __device__ __forceinline__ int64_t rope_row(int64_t p, int64_t rows) {
 // launch, so launches captured into a CUDA graph make no attribute calls after the first.
 cudaError_t ensure_smem(const void* kernel, int bytes);
 
+// Count one kernel launch (dsv41_launch_count).
+void count_launch();
+
 }  // namespace dsv41

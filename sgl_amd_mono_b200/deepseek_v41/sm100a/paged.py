@@ -1,0 +1,177 @@
+"""A paged 8-bit cache of grouped-query keys and values, and the two operators of a decode step on
+it: the append of the step's rows (with the position rotation) and their attention.
+
+``PagedKV`` wraps the cache's four tensors, which a server allocates once: keys and values
+``[pages, kv_heads, page, dim]`` e4m3 bytes, and an E8M0 code per ``block`` consecutive tokens of a
+head, ``[pages, kv_heads, page / block]``. Sequence ``s`` of a step holds ``lens[s]`` tokens on the
+pages ``table[s]``; its rows are its last tokens. The rows ``[T, heads, dim]`` of all sequences lie
+one after the other: ``cu_rows[s] .. cu_rows[s + 1]`` are sequence ``s``'s, or row ``s`` alone with
+``cu_rows=None``. Everything a call needs stays on the device, so a call can be captured in a CUDA
+graph with its lengths and pages changed between replays; a padded batch gives its unused
+sequences no rows (or length 0). Host-side argument errors raise ``RuntimeError``.
+"""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from ...common import ext
+from . import abi
+
+DIMS = (64, 128, 256)
+
+
+def check_device(device: torch.device, name: str) -> None:
+    """Raise unless ``device`` is the current CUDA device, whose stream the launch goes to."""
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise RuntimeError(f"{name}: on {device}, which is not the current CUDA device")
+
+
+class PagedKV:
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor):
+        if k.dim() != 4 or k_codes.dim() != 3:
+            raise RuntimeError(f"PagedKV: keys {tuple(k.shape)}, codes {tuple(k_codes.shape)}; want "
+                               "[pages, kv_heads, page, dim] and [pages, kv_heads, page / block]")
+        pages, heads, page, dim = k.shape
+        per = k_codes.shape[2]
+        if dim not in DIMS or not pages or not heads or not per or page % per or page // per % 16 or not page:
+            raise RuntimeError(f"PagedKV: pages {pages}, heads {heads}, page {page}, dim {dim}, {per} codes a page: "
+                               f"dim in {DIMS}, tokens a code a multiple of 16")
+        for t, name, shape in ((k, "keys", k.shape), (v, "values", k.shape),
+                               (k_codes, "key codes", (pages, heads, per)), (v_codes, "value codes", (pages, heads, per))):
+            if t.shape != tuple(shape) or t.element_size() != 1 or not t.is_contiguous() or t.device != k.device:
+                raise RuntimeError(f"PagedKV: {name} {tuple(t.shape)} {t.dtype} on {t.device}: want contiguous bytes "
+                                   f"{tuple(shape)} on {k.device}")
+        self.k, self.v, self.k_codes, self.v_codes = k, v, k_codes, v_codes
+        self.pages, self.kv_heads, self.page, self.dim, self.block = pages, heads, page, dim, page // per
+        cache = dict(kv_heads=heads, dim=dim, k_cache=k.data_ptr(), v_cache=v.data_ptr(), k_codes=k_codes.data_ptr(),
+                     v_codes=v_codes.data_ptr(), pages=pages, page=page, block=self.block)
+        self._append_args, self._attend_args = abi.KvAppendArgs(**cache), abi.PagedAttnArgs(**cache)
+
+    @classmethod
+    def empty(cls, pages: int, page: int, kv_heads: int, dim: int, *, block: int = 16, device="cuda") -> "PagedKV":
+        """A new cache of ``pages`` pages of ``page`` tokens."""
+        if block < 16 or block % 16 or page % block:
+            raise RuntimeError(f"PagedKV: page {page}, block {block}: block a multiple of 16, page of block")
+        u8 = dict(dtype=torch.uint8, device=device)
+        data, codes = (pages, kv_heads, page, dim), (pages, kv_heads, page // block)
+        return cls(torch.zeros(data, **u8), torch.zeros(data, **u8), torch.zeros(codes, **u8),
+                   torch.zeros(codes, **u8))
+
+    # ------------------------------------------------------------ checks
+    def _rows(self, x: torch.Tensor, name: str, like: torch.Tensor, heads: int | None = None) -> int:
+        """Check rows [T, heads, dim] (a row's heads contiguous) and return their stride."""
+        shape, st = x.shape, x.stride()
+        if (len(shape) != 3 or shape[0] != like.shape[0] or shape[2] != self.dim or x.dtype != like.dtype
+                or (heads is not None and shape[1] != heads) or x.device != self.k.device):
+            raise RuntimeError(f"{name}: {tuple(shape)} {x.dtype} on {x.device}: want [{like.shape[0]}, "
+                               f"{heads or 'heads'}, {self.dim}] {like.dtype} on {self.k.device}")
+        ld = st[0] if shape[0] > 1 else max(st[0], shape[1] * self.dim)
+        ld = ld if shape[0] > 1 else -(-ld // 8) * 8
+        if st[2] != 1 or (st[1] != self.dim and shape[1] > 1) or ld % 8 or ld < shape[1] * self.dim \
+                or x.data_ptr() % 16:
+            raise RuntimeError(f"{name}: strides {st} at {x.data_ptr():#x}: a row's heads have to be contiguous, rows "
+                               "a multiple of 8 values apart and 16-byte aligned")
+        return ld
+
+    def _step(self, a, x: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, cu_rows: torch.Tensor | None) -> None:
+        """Check the step's tensors and fill in what the two calls share."""
+        dev = self.k.device
+        check_device(dev, "PagedKV")
+        if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
+            raise RuntimeError(f"PagedKV: rows of {x.dtype}, want bfloat16 or float16")
+        i32 = torch.int32
+        seqs = lens.shape[0] if lens.dim() == 1 else -1
+        if seqs < 0 or lens.dtype != i32 or lens.device != dev or not lens.is_contiguous():
+            raise RuntimeError(f"lens: {tuple(lens.shape)} {lens.dtype} on {lens.device}: want [sequences] int32 on {dev}")
+        if table.dim() != 2 or table.shape[0] != seqs or table.shape[1] < 1 or table.dtype != i32 \
+                or table.device != dev or table.stride(1) != 1 or (seqs > 1 and table.stride(0) < table.shape[1]):
+            raise RuntimeError(f"table: {tuple(table.shape)} {table.dtype} on {table.device}: want [{seqs}, pages] int32 "
+                               f"with contiguous rows on {dev}")
+        if cu_rows is None:
+            if seqs != x.shape[0]:
+                raise RuntimeError(f"{x.shape[0]} rows for {seqs} sequences without cu_rows: one row a sequence")
+        elif cu_rows.shape != (seqs + 1,) or cu_rows.dtype != i32 or cu_rows.device != dev \
+                or not cu_rows.is_contiguous():
+            raise RuntimeError(f"cu_rows: {tuple(cu_rows.shape)} {cu_rows.dtype} on {cu_rows.device}: want [{seqs + 1}] "
+                               f"int32 on {dev}")
+        a.T, a.seqs, a.f16 = x.shape[0], seqs, x.dtype is torch.float16
+        a.lens, a.table, a.width = lens.data_ptr(), table.data_ptr(), table.shape[1]
+        a.table_ld = max(table.stride(0), a.width)
+        a.cu_rows = 0 if cu_rows is None else cu_rows.data_ptr()
+
+    # ------------------------------------------------------------ operators
+    def append(self, k: torch.Tensor, v: torch.Tensor, *, lens: torch.Tensor, table: torch.Tensor,
+               cu_rows: torch.Tensor | None = None, q: torch.Tensor | None = None,
+               cos_sin: torch.Tensor | None = None, neox: bool = False,
+               q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Write the step's keys and values [T, kv_heads, dim] (bf16 or f16) into the cache as its
+        sequences' last tokens; ``lens`` [sequences] int32 counts them already. With ``cos_sin``
+        [positions, rope] fp32 (rope / 2 cos, then rope / 2 sin) the last ``rope`` dims of the keys,
+        and of the queries ``q`` [T, heads, dim] where given, are rotated by their positions, in
+        pairs (2j, 2j + 1) or, ``neox``, (j, j + rope / 2). Returns the rotated queries (``q_out``,
+        which may be ``q``, or a new tensor), or None without ``q``. A sequence's pages must not be
+        another's: two sequences that append to one block race."""
+        a = abi.KvAppendArgs.from_buffer_copy(self._append_args)
+        if k.dim() != 3:
+            raise RuntimeError(f"k: {tuple(k.shape)}: want [rows, {self.kv_heads}, {self.dim}]")
+        self._step(a, k, lens, table, cu_rows)
+        a.k, a.k_ld = k.data_ptr(), self._rows(k, "k", k, self.kv_heads)
+        a.v, a.v_ld = v.data_ptr(), self._rows(v, "v", k, self.kv_heads)
+        a.heads = self.kv_heads
+        if cos_sin is not None:
+            if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.device != self.k.device \
+                    or not cos_sin.is_contiguous() or not cos_sin.shape[0] or cos_sin.shape[1] % 16 \
+                    or not 16 <= cos_sin.shape[1] <= self.dim or cos_sin.data_ptr() % 16:
+                raise RuntimeError(f"cos_sin: {tuple(cos_sin.shape)} {cos_sin.dtype} on {cos_sin.device}: want "
+                                   f"[positions, rope] fp32, rope a multiple of 16 up to {self.dim}")
+            a.cos_sin, a.rope_rows, a.rope, a.neox = cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1], bool(neox)
+        if q is not None:
+            a.q, a.q_ld = q.data_ptr(), self._rows(q, "q", k)
+            a.heads = q.shape[1]
+            if not a.heads or a.heads % self.kv_heads:
+                raise RuntimeError(f"q: {a.heads} heads over {self.kv_heads} key heads")
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            a.q_out, a.q_out_ld = q_out.data_ptr(), self._rows(q_out, "q_out", k, a.heads)
+        elif q_out is not None:
+            raise RuntimeError("q_out without q")
+        ext.call("dsv41_kv_append", a, torch.cuda.current_stream().cuda_stream)
+        return q_out
+
+    def attend(self, q: torch.Tensor, *, lens: torch.Tensor, table: torch.Tensor, scale: float,
+               cu_rows: torch.Tensor | None = None, window: int = 0, sink: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the rows q [T, heads, dim] (bf16 or f16) over the cache: row j of a
+        sequence's n sees the tokens before ``lens[s] - n + j + 1`` (causal over the step's own
+        rows), with ``window`` the last ``window`` of them; ``scale`` times q . k goes into the
+        softmax, with ``sink`` [heads] fp32 as one more score without a value. A row that sees
+        nothing gives zeros. Returns ``out`` (or a new tensor) [T, heads, dim]; rows behind the last
+        sequence are left as they were."""
+        a = abi.PagedAttnArgs.from_buffer_copy(self._attend_args)
+        if q.dim() != 3:
+            raise RuntimeError(f"q: {tuple(q.shape)}: want [rows, heads, {self.dim}]")
+        self._step(a, q, lens, table, cu_rows)
+        a.q, a.q_ld = q.data_ptr(), self._rows(q, "q", q)
+        a.heads = heads = q.shape[1]
+        if not heads or heads % self.kv_heads:
+            raise RuntimeError(f"q: {heads} heads over {self.kv_heads} key heads")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        a.out, a.out_ld = out.data_ptr(), self._rows(out, "out", q, heads)
+        if not 0 <= window < 1 << 31:
+            raise RuntimeError(f"window {window}")
+        a.window = window
+        if sink is not None:
+            if sink.shape != (heads,) or sink.dtype != torch.float32 or sink.device != q.device \
+                    or not sink.is_contiguous():
+                raise RuntimeError(f"sink: {tuple(sink.shape)} {sink.dtype} on {sink.device}: want [{heads}] fp32")
+            a.sink = sink.data_ptr()
+        a.scale_f32 = struct.unpack("<I", struct.pack("<f", scale))[0]
+        need = ext.query("dsv41_paged_attn_scratch_bytes", a)
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.scratch, a.scratch_bytes = scratch.data_ptr(), need
+        ext.call("dsv41_paged_attn", a, torch.cuda.current_stream().cuda_stream)
+        return out
