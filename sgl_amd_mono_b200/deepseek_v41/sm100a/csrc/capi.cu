@@ -821,6 +821,8 @@ int k2_run(const Dsv41K2Args* a, cudaStream_t st, bool go, int64_t* need) {
 }  // namespace
 
 void dsv41::count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+int dsv41::device_sms() { return sm_count(); }
+bool dsv41::pdl_on() { return use_pdl(); }
 
 extern "C" {
 

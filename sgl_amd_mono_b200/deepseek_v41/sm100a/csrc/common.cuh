@@ -292,7 +292,10 @@ __device__ __forceinline__ int64_t rope_row(int64_t p, int64_t rows) {
 // launch, so launches captured into a CUDA graph make no attribute calls after the first.
 cudaError_t ensure_smem(const void* kernel, int bytes);
 
-// Count one kernel launch (dsv41_launch_count).
+// Count one kernel launch (dsv41_launch_count); the current device's SMs; whether launches use
+// programmatic dependent launch (dsv41_set_option "pdl").
 void count_launch();
+int device_sms();
+bool pdl_on();
 
 }  // namespace dsv41

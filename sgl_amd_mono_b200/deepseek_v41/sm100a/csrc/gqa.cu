@@ -1,9 +1,11 @@
 // extern "C" entry points of the grouped-query decode operators (include/dsv41_b200.h): the 4-bit
 // GEMV, the paged 8-bit cache's append and the attention over it. Argument checks, then the launches
 // on the caller's stream.
+#include <algorithm>
 #include <climits>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "../../../../include/dsv41_b200.h"
 #include "gemv_w4.cuh"
@@ -20,15 +22,31 @@ T* ptr(int64_t v) {
   return reinterpret_cast<T*>(v);
 }
 
+// One launch with programmatic dependent launch (every kernel waits before it reads).
 template <class Args>
 int launch(void (*kernel)(const Args), dim3 grid, dim3 block, int smem, void* stream, const Args& args) {
-  count_launch();
-  kernel<<<grid, block, smem, reinterpret_cast<cudaStream_t>(stream)>>>(args);
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e = smem > 48 * 1024 ? ensure_smem(reinterpret_cast<const void*>(kernel), smem) : cudaSuccess;
+  if (e == cudaSuccess) {
+    count_launch();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_on() ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, args);
+  }
   if (e == cudaSuccess) return DSV41_OK;
+  cudaGetLastError();
   fprintf(stderr, "dsv41: launch failed: %s\n", cudaGetErrorString(e));
   return DSV41_ELAUNCH;
 }
+
+int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Rows [T, heads, dim] of 2-byte values, ld elements apart.
 bool rows_ok(int64_t p, int64_t ld, int64_t heads, int64_t dim) {
@@ -72,6 +90,56 @@ bool attn_ok(const Dsv41PagedAttnArgs* a) {
          a->window >= 0 && a->window <= INT_MAX && a->sink % 4 == 0;
 }
 
+// Columns of 8 a CTA takes together. A sequence's columns (its rows times the query heads of a kv
+// head; T / seqs rows on average) share every key that is read, so as many as they fill, up to the
+// accumulators that fit: 32 columns of 64 or 128 dims, 16 of 256.
+int attn_tiles(const Dsv41PagedAttnArgs* a) {
+  const int64_t cols = a->heads / a->kv_heads * std::max<int64_t>(1, cdiv64(a->T, std::max<int64_t>(1, a->seqs)));
+  return cols <= 8 ? 1 : cols <= 16 || a->dim == 256 ? 2 : 4;
+}
+
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+// f(type, dim, column tiles) of the arguments' kernel.
+template <class F>
+int64_t attn_go(const Dsv41PagedAttnArgs* a, F f) {
+  auto by_type = [&](auto d, auto nt) { return a->f16 ? f(Int<1>(), d, nt) : f(Int<0>(), d, nt); };
+  auto by_tiles = [&](auto d) {
+    switch (attn_tiles(a)) {
+      case 1: return by_type(d, Int<1>());
+      case 2: return by_type(d, Int<2>());
+      default: return by_type(d, Int<d == 256 ? 2 : 4>());
+    }
+  };
+  return a->dim == 64 ? by_tiles(Int<64>()) : a->dim == 128 ? by_tiles(Int<128>()) : by_tiles(Int<256>());
+}
+
+template <int D, int NT>
+int64_t attn_ctas() {
+  return (int64_t)device_sms() * PaShape<D, NT>::kCtas;
+}
+template <int D, int NT>
+int64_t attn_scratch() {
+  return 2 * attn_ctas<D, NT>() * 8 * NT * (D * sizeof(float) + sizeof(float4));
+}
+
+template <int F16, int D, int NT>
+int attn_run(const Dsv41PagedAttnArgs* a, void* stream) {
+  if (!a->scratch || a->scratch % 16 || a->scratch_bytes < attn_scratch<D, NT>()) return DSV41_ESCRATCH;
+  const uint32_t bits = (uint32_t)a->scale_f32;
+  float scale;
+  memcpy(&scale, &bits, 4);
+  const int64_t ctas = attn_ctas<D, NT>(), slots = 2 * ctas * 8 * NT;
+  float* part = ptr<float>(a->scratch);
+  const PagedAttnArgs p = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->window, scale * 1.44269504f,
+                           ptr<const void>(a->q), ptr<void>(a->out), a->q_ld, a->out_ld, ptr<const float>(a->sink),
+                           part, reinterpret_cast<float4*>(part + slots * D)};
+  const int rc = launch(paged_attn_kernel<F16, D, NT>, dim3((unsigned)ctas), dim3(32 * kPaWarps),
+                        PaShape<D, NT>::kBytes, stream, p);
+  return rc ? rc : launch(paged_join_kernel<F16, D, NT>, dim3((unsigned)ctas), dim3(32 * kPaWarps), 0, stream, p);
+}
+
 bool w4_ok(const Dsv41GemvW4Args* a) {
   return a && a->w && a->w % 16 == 0 && a->scales && a->scales % 2 == 0 && a->x && a->x % 16 == 0 && a->y &&
          a->y % 2 == 0 && a->M >= 1 && a->M <= kW4MaxRows && a->N >= 1 && a->N <= (1 << 24) && a->group >= 32 &&
@@ -109,25 +177,15 @@ int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
   }
 }
 
-int64_t dsv41_paged_attn_scratch_bytes(const Dsv41PagedAttnArgs* a) { return attn_ok(a) ? 0 : DSV41_EINVAL; }
+int64_t dsv41_paged_attn_scratch_bytes(const Dsv41PagedAttnArgs* a) {
+  if (!attn_ok(a)) return DSV41_EINVAL;
+  return attn_go(a, [](auto, auto d, auto nt) { return attn_scratch<d, nt>(); });
+}
 
 int dsv41_paged_attn(const Dsv41PagedAttnArgs* a, void* stream) {
   if (!attn_ok(a)) return DSV41_EINVAL;
   if (!a->T || !a->seqs) return DSV41_OK;
-  const uint32_t bits = (uint32_t)a->scale_f32;
-  float scale;
-  memcpy(&scale, &bits, 4);
-  const PagedAttnArgs p = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->window, scale, ptr<const void>(a->q),
-                           ptr<void>(a->out), a->q_ld, a->out_ld, ptr<const float>(a->sink)};
-  const dim3 grid(p.rows.T, cdiv(p.heads, 4));
-  switch (a->dim * 2 + a->f16) {
-    case 128: return launch(paged_attn_kernel<false, 64>, grid, dim3(128), 0, stream, p);
-    case 129: return launch(paged_attn_kernel<true, 64>, grid, dim3(128), 0, stream, p);
-    case 256: return launch(paged_attn_kernel<false, 128>, grid, dim3(128), 0, stream, p);
-    case 257: return launch(paged_attn_kernel<true, 128>, grid, dim3(128), 0, stream, p);
-    case 512: return launch(paged_attn_kernel<false, 256>, grid, dim3(128), 0, stream, p);
-    default: return launch(paged_attn_kernel<true, 256>, grid, dim3(128), 0, stream, p);
-  }
+  return (int)attn_go(a, [&](auto f16, auto d, auto nt) { return (int64_t)attn_run<f16, d, nt>(a, stream); });
 }
 
 }  // extern "C"

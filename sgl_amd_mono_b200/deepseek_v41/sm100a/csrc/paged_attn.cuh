@@ -1,65 +1,661 @@
-// Attention of decode and verify rows over the paged e4m3 cache (dsv41_paged_attn): per row and
-// query head o = sum_i softmax(scale q . k_i)_i v_i over the keys the row sees, in one pass with the
-// running maximum m and sum l of the softmax in fp32.
+// Attention of decode and verify rows over the paged e4m3 cache (dsv41_paged_attn).
+//
+// Mathematics. For a row's query head with scores s_i = scale q . k_i (base 2: scale log2 e), keys
+// k_i = 2^a_i K_i and values v_i = 2^b_i V_i (K, V e4m3 bytes, a and b one power of two per block
+// of tokens and head): o = 2^(r - c) sum_i 2^(s_i + b_i - r) V_i / sum_i 2^(s_i - c), one pass with
+// two running references. The value's scale goes into the weight's exponent, so the weights w_i =
+// 2^(s_i + b_i - r + 7) multiply raw bytes; r follows the largest s_i + b_i seen, c the largest s_i
+// (two, since a scale may be any power of two: one reference could overflow the sum). Both move only
+// when a weight would pass 2^15 (or a term of the sum 2^60), so most tiles rescale nothing.
+//
+// Layout. What bounds the kernel is reading the cache once, so all columns (a sequence's rows times
+// the query heads of a kv head) that fit share each tile. A tile is 16 tokens of one kv head: 16 dim
+// contiguous bytes of K and of V, never across a page or a scale block. A warp streams its own tiles
+// through its own ring of shared memory by 16-byte cp.async, with no barrier between warps; S^T = K
+// Q^T puts the 16 tokens in the m16n8k16 rows and 8 columns in N, so a group of 8 heads or fewer
+// wastes little, and O^T = V^T P^T takes P from S's registers by a transposing movmatrix.
+//
+// Roundings. K and V become f16 exactly; q is scaled per column by a power of two into f16's range
+// (exact but for values 2^-29 below the column's largest). Scores, weights, sums and O are fp32; only
+// the weights are rounded to f16 for the second product: half a step of 2^-11 of each weight, and
+// those below 2^-21 of the largest keep an absolute 2^-32 of it.
+//
+// Split. The work (sequence, kv head, column tile, steps of 16 W tokens) is cut into equal
+// contiguous shares, one a CTA, whatever the lengths: each CTA finds its own from the lengths on the
+// device. A share's piece of an item that lies in several shares goes to scratch, and a second kernel
+// joins the pieces in order, so the sums do not depend on timing.
 #pragma once
+
+#include <cfloat>
 
 #include "gqa.cuh"
 
 namespace dsv41 {
 
+constexpr int kPaWarps = 8;
+
 struct PagedAttnArgs {
   StepRows rows;
   KvCache cache;
   int heads, window;
-  float scale;
+  float scale;  // times log2 e
   const void* q;
   void* out;
   int64_t q_ld, out_ld;
   const float* sink;  // [heads] or null
+  float* part;        // [2 CTAs][8 NT][dim] unnormalised pieces
+  float4* part_rl;    // [2 CTAs][8 NT] their references r and c and their sum
 };
 
-// Grid (T, ceil(heads / 4)), 128 threads: a warp a (row, query head), key by key.
-template <bool F16, int D>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) {
-  using T = typename Act<F16>::T;
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int r = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (h >= a.heads) return;
-  const int seq = row_seq(a.rows, r, lane);
-  if (seq < 0) return;
-  const int first = a.rows.cu_rows ? a.rows.cu_rows[seq] : r;
-  const int n = a.rows.cu_rows ? a.rows.cu_rows[seq + 1] - first : 1;
-  const int page = a.cache.page, block = a.cache.block, kvh = a.cache.kv_heads;
-  const int vis = (int)min((int64_t)a.rows.lens[seq] - n + (r - first) + 1, (int64_t)a.rows.width * page);
-  const int lo = a.window ? max(0, a.rows.lens[seq] - n + (r - first) + 1 - a.window) : 0;
-  const int hk = h / (a.heads / kvh);
-  const T* qp = reinterpret_cast<const T*>(a.q) + r * a.q_ld + h * D;
-  float q[D / 32], o[D / 32];
+// One sequence's work: its rows, its tiles [tile0, tile0 + tiles) and what that makes in units.
+struct SeqWork {
+  int row0, n, cols, cts, tile0, tiles, steps, end;  // end: tokens its last row sees (unclamped)
+  long long units;
+};
+
+template <int NT>
+__device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
+  SeqWork w;
+  w.row0 = a.rows.cu_rows ? a.rows.cu_rows[s] : s;
+  w.n = a.rows.cu_rows ? a.rows.cu_rows[s + 1] - w.row0 : 1;
+  w.n = w.row0 < 0 || w.row0 > a.rows.T ? 0 : max(0, min(w.n, a.rows.T - w.row0));
+  w.end = a.rows.lens[s];
+  const int kvh = a.cache.kv_heads;
+  w.cols = w.n * (a.heads / kvh);
+  w.cts = (w.cols + 8 * NT - 1) / (8 * NT);
+  const int hi = min(max(w.end, 0), a.rows.width * a.cache.page);
+  const int lo = a.window ? max(0, w.end - w.n + 1 - a.window) : 0;
+  w.tile0 = lo / 16;
+  w.tiles = max(0, (hi + 15) / 16 - w.tile0);
+  w.steps = max(1, (w.tiles + kPaWarps - 1) / kPaWarps);
+  w.units = (long long)w.cts * kvh * w.steps;
+  return w;
+}
+
+// The whole work and this share of it: seq and unit where share `c` of `shares` begins, found by all
+// threads of a 32 kPaWarps CTA. per = units a share.
+struct Share {
+  long long first, last, per;  // units [first, last)
+  int seq;                     // the sequence of unit `first`
+  long long seq0;              // its first unit
+};
+
+template <int NT>
+__device__ __forceinline__ Share find_share(const PagedAttnArgs& a, int c, int shares, long long* sm) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kThreads = 32 * kPaWarps;
+  const int seqs = a.rows.seqs;
+  // the units before each thread's sequence, a chunk of kThreads sequences at a time
+  auto scan = [&](int base, long long& before, long long& own) {
+    own = base + tid < seqs ? seq_work<NT>(a, base + tid).units : 0;
+    long long x = own;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) q[i] = Act<F16>::f(qp[lane + 32 * i]), o[i] = 0.f;
-  float m = a.sink ? a.sink[h] : -INFINITY, l = a.sink ? 1.f : 0.f;
-  for (int p = lo; p < vis; ++p) {
-    const int pg = token_page(a.rows, a.cache, seq, p);
-    if (pg < 0) continue;
-    const int64_t head = (int64_t)pg * kvh + hk;
-    const uint8_t* kp = a.cache.k + (head * page + p % page) * D;
-    const uint8_t* vp = a.cache.v + (head * page + p % page) * D;
-    const int64_t ci = head * (page / block) + p % page / block;
-    float s = 0.f;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sm[warp] = x;
+    __syncthreads();
+    before = x - own;
+    long long all = 0;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) s += q[i] * e4m3_float(kp[lane + 32 * i]);
-    s = warp_sum(s) * pow2c(a.cache.k_codes[ci]) * a.scale;
-    const float mn = fmaxf(m, s), f = m == mn ? 1.f : __expf(m - mn), w = __expf(s - mn);
-    const float vs = w * pow2c(a.cache.v_codes[ci]);
-    l = l * f + w;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * f + vs * e4m3_float(vp[lane + 32 * i]);
-    m = mn;
+    for (int i = 0; i < kPaWarps; ++i) {
+      if (i < warp) before += sm[i];
+      all += sm[i];
+    }
+    return all;
+  };
+  long long before, own, total = scan(0, before, own);
+  for (int base = kThreads; base < seqs; base += kThreads) {
+    long long b, o;
+    total += scan(base, b, o);
   }
-  T* y = reinterpret_cast<T*>(a.out) + r * a.out_ld + h * D;
+  Share r;
+  r.per = (total + shares - 1) / shares;
+  r.first = c * r.per;
+  r.last = min(r.first + r.per, total);
+  if (r.first >= total) return r.seq = -1, r;
+  __syncthreads();
+  long long sum = 0;
+  for (int base = 0; base < seqs; base += kThreads) {
+    if (seqs > kThreads) {
+      const long long all = scan(base, before, own);
+      before += sum;
+      sum += all;
+    }
+    if (own && before <= r.first && r.first < before + own) {
+      sm[kPaWarps] = base + tid;
+      sm[kPaWarps + 1] = before;
+    }
+  }
+  __syncthreads();
+  r.seq = (int)sm[kPaWarps];
+  r.seq0 = sm[kPaWarps + 1];
+  return r;
+}
+
+// A tile's token rows in the mma's M order: row g is token kappa(g) (g + 8: 8 more). With the
+// swizzle below every shared-memory read of K and V is free of bank conflicts.
+__device__ __forceinline__ int pa_kappa(int g) { return (g & 1) ? 7 - (g >> 1) : g >> 1; }
+// Where 16-byte chunk c of token row `row` lies in a staged tile.
+template <int D>
+__device__ __forceinline__ uint32_t pa_chunk(int row, int c) {
+  return row * D + ((D == 64 ? c ^ (row & 2) : c ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// f16x2 of the low and of the high two e4m3 bytes of w (exact, NaN kept).
+__device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+// Whether a byte of w is an e4m3 NaN.
+__device__ __forceinline__ bool has_nan(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
+
+template <int D, int NT>
+struct PaShape {
+  static constexpr int kRegs = NT * D;              // O registers a thread: kRegs / 4
+  static constexpr int kCtas = kRegs <= 128 ? 2 : 1;  // an SM
+  static constexpr int kTile = 32 * D;              // bytes of a staged tile, K and V
+  static constexpr int kStagesFit = (kCtas == 2 ? 96 : 192) * 1024 / (kPaWarps * kTile);
+  static constexpr int kStages = kStagesFit > 6 ? 6 : kStagesFit;
+  static constexpr bool kQSmem = kRegs > 256;       // Q fragments re-read from shared memory
+  static constexpr int kRing = kPaWarps * kStages * kTile;
+  static constexpr int kQBytes = kQSmem ? 8 * NT * D * 2 : 0;
+  static constexpr int kRl = kPaWarps * 8 * NT * 16;  // the warps' references and sums
+  static constexpr int kBytes = kRing + kQBytes + kRl + (kPaWarps + 2) * 8;
+  static_assert(kPaWarps / 2 * 8 * NT * D * 4 <= kRing, "the merge reuses the ring");
+};
+
+// What turns sum_i w_i V_i into the output: 2^(r - 7 - c) over the sum (0 where nothing was seen).
+__device__ __forceinline__ float pa_factor(float ref, float top, float sum) {
+  return sum == 0.f ? 0.f : ex2(ref - top - 7.f) / sum;
+}
+
+// out[8 dims] of one column from 8 consecutive values.
+template <bool F16>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(Act<F16>::pack(v[0], v[1]), Act<F16>::pack(v[2], v[3]), Act<F16>::pack(v[4], v[5]),
+                    Act<F16>::pack(v[6], v[7]));
+}
+
+template <bool F16, int D, int NT>
+__global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_attn_kernel(const PagedAttnArgs a) {
+  using P = PaShape<D, NT>;
+  using T = typename Act<F16>::T;
+  constexpr int W = kPaWarps, S = P::kStages, KS = D / 16;
+  extern __shared__ __align__(128) uint8_t pa_smem[];
+  uint2* q_sm = reinterpret_cast<uint2*>(pa_smem + P::kRing);
+  float4* rl_sm = reinterpret_cast<float4*>(pa_smem + P::kRing + P::kQBytes);
+  long long* plan_sm = reinterpret_cast<long long*>(pa_smem + P::kRing + P::kQBytes + P::kRl);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(pa_smem) + warp * S * P::kTile;
+  const int kvh = a.cache.kv_heads, group = a.heads / kvh, page = a.cache.page, block = a.cache.block;
+  const int kap = pa_kappa(g);
+
+  pdl_wait();
+  pdl_launch();
+  const Share sh = find_share<NT>(a, blockIdx.x, gridDim.x, plan_sm);
+  if (sh.seq < 0) return;
+  int seq = sh.seq;
+  SeqWork w = seq_work<NT>(a, seq);
+  long long seq0 = sh.seq0;
+  for (long long u = sh.first; u < sh.last;) {
+    while (u >= seq0 + w.units) {
+      seq0 += w.units;
+      w = seq_work<NT>(a, ++seq);
+    }
+    // this piece: kv head hk, column tile ct, steps [step0, step1)
+    const int item = (int)((u - seq0) / w.steps), step0 = (int)((u - seq0) % w.steps);
+    const int step1 = (int)min((long long)w.steps, step0 + sh.last - u);
+    const int ct = item % w.cts, hk = item / w.cts;
+    const int col0 = ct * 8 * NT;
+    // what its first and last row see
+    const int j0 = col0 / group, j1 = (min(col0 + 8 * NT, w.cols) - 1) / group;
+    const int cap = a.rows.width * page;
+    auto vis = [&](int j) { return w.end - w.n + j + 1; };
+    auto low = [&](int j) { return a.window ? max(0, vis(j) - a.window) : 0; };
+    const int any_lo = low(j0), any_hi = min(vis(j1), cap), all_lo = low(j1), all_hi = min(vis(j0), cap);
+
+    // Q: column n's dims 64 c + 16 t + 4 q + {0 .. 3} are step 4 c + q's fragment of lane (n, t)
+    uint32_t qf[P::kQSmem ? 1 : NT][P::kQSmem ? 1 : KS][2];
+    float qmul[NT][2];
+    if (P::kQSmem) __syncthreads();
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) y[lane + 32 * i] = Act<F16>::r(l == 0.f ? 0.f : o[i] / l);
+    for (int n = 0; n < NT; ++n) {
+      const int col = col0 + 8 * n + g;
+      uint32_t raw[KS][2];
+      float amax = 0.f;
+      const T* qp = reinterpret_cast<const T*>(a.q) + (w.row0 + col / group) * a.q_ld + (hk * group + col % group) * D;
+      if (!P::kQSmem || warp == n % W) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint4 x[2] = {};
+          if (col < w.cols) {
+            x[0] = ldg16(qp + 64 * c + 16 * t);
+            x[1] = ldg16(qp + 64 * c + 16 * t + 8);
+          }
+          const uint32_t v[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            raw[4 * c + i / 2][i & 1] = v[i];
+            if (!F16) {
+              const float2 f = Act<F16>::unpack(v[i]);
+              amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+        }
+      }
+      float inv = 1.f;
+      if (!F16) {
+        // scale the column so that its largest value is below 2^14
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        int e = (int)((__float_as_uint(amax) >> 23) & 255);
+        e = e == 255 ? 127 + 13 : max(e, 40);
+        const float mul = __uint_as_float((uint32_t)(254 + 13 - e) << 23);
+        inv = __uint_as_float((uint32_t)(e - 13) << 23);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 f = Act<F16>::unpack(raw[k][i]);
+            raw[k][i] = pack_f16x2(f.x * mul, f.y * mul);
+          }
+      }
+      if (P::kQSmem) {
+        if (warp == n % W) {
+#pragma unroll
+          for (int k = 0; k < KS; ++k) q_sm[(n * KS + k) * 32 + lane] = make_uint2(raw[k][0], raw[k][1]);
+          if (t == 0) rl_sm[8 * n + g].x = inv;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) qf[n][k][0] = raw[k][0], qf[n][k][1] = raw[k][1];
+        qmul[n][0] = __shfl_sync(0xffffffffu, inv, 8 * t) * a.scale;
+        qmul[n][1] = __shfl_sync(0xffffffffu, inv, 8 * t + 4) * a.scale;
+      }
+    }
+    if (P::kQSmem) {
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) qmul[n][e] = rl_sm[8 * n + 2 * t + e].x * a.scale;
+    }
+
+    float o[NT][KS][4], ref[NT][2], top[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+      ref[n][0] = ref[n][1] = top[n][0] = top[n][1] = -FLT_MAX;
+      l[n][0] = l[n][1] = 0.f;
+    }
+
+    // the warp's tiles: w.tile0 + first + W j, j < count
+    const int first = step0 * W + warp;
+    const int count = max(0, (min(step1 * W, w.tiles) - first + W - 1) / W);
+    // lane i holds page and scale codes of tile 32 b + i of the batch being issued (cur) and of the
+    // one before (prev): page, or -1 where the piece sees none of the tile's tokens
+    int cur_pg = -1, prev_pg = -1;
+    uint32_t cur_sc = 0, prev_sc = 0;
+    auto load_batch = [&](int b) {
+      prev_pg = cur_pg, prev_sc = cur_sc;
+      const int j = 32 * b + lane, p0 = (w.tile0 + first + W * j) * 16;
+      cur_pg = -1;
+      if (j < count && p0 < any_hi && p0 + 16 > any_lo) {
+        cur_pg = token_page(a.rows, a.cache, seq, p0);
+        if (cur_pg >= 0) {
+          const int64_t ci = ((int64_t)cur_pg * kvh + hk) * (page / block) + p0 % page / block;
+          cur_sc = a.cache.k_codes[ci] | ((uint32_t)a.cache.v_codes[ci] << 8);
+        }
+      }
+    };
+    auto issue = [&](int j) {
+      if (j < count) {
+        if (j % 32 == 0) load_batch(j / 32);
+        const int pg = __shfl_sync(0xffffffffu, cur_pg, j & 31);
+        if (pg >= 0) {
+          const int64_t at = (((int64_t)pg * kvh + hk) * page + (w.tile0 + first + W * j) * 16 % page) * D;
+          const uint32_t dst = ring + j % S * P::kTile;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const int idx = lane + 32 * i;
+            const uint32_t d = dst + pa_chunk<D>(idx / (D / 16), idx % (D / 16));
+            cp_async16_stream(d, a.cache.k + at + idx * 16);
+            cp_async16_stream(d + 16 * D, a.cache.v + at + idx * 16);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll 1
+    for (int j = 0; j < S - 1; ++j) issue(j);
+#pragma unroll 1
+    for (int j = 0; j < count; ++j) {
+      issue(j + S - 1);
+      cp_async_wait<S - 1>();
+      __syncwarp();
+      // batch j / 32 is cur, or prev once the issue has gone on to the next
+      const bool is_cur = min(j + S - 1, count - 1) / 32 == j / 32;
+      const int pg = __shfl_sync(0xffffffffu, is_cur ? cur_pg : prev_pg, j & 31);
+      const uint32_t sc = __shfl_sync(0xffffffffu, is_cur ? cur_sc : prev_sc, j & 31);
+      if (pg < 0) continue;
+      const uint32_t kt = ring + j % S * P::kTile, vt = kt + 16 * D;
+      const int p0 = (w.tile0 + first + W * j) * 16;
+      const bool edge = p0 < all_lo || p0 + 16 > all_hi;
+
+      // S^T = K Q^T
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        const uint4 x = lds16(kt + pa_chunk<D>(kap, 4 * c + t)), y = lds16(kt + pa_chunk<D>(kap + 8, 4 * c + t));
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_f16(xs[i], a0, a2);
+          e4m3x4_f16(ys[i], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint2 b;
+            if (P::kQSmem) b = q_sm[(n * KS + 4 * c + i) * 32 + lane];
+            else b = make_uint2(qf[P::kQSmem ? 0 : n][P::kQSmem ? 0 : 4 * c + i][0],
+                                qf[P::kQSmem ? 0 : n][P::kQSmem ? 0 : 4 * c + i][1]);
+            mma_f16(s[n], a0, a1, a2, a3, b.x, b.y);
+          }
+        }
+      }
+
+      // s: scores, base 2; elements (token kappa, column 2t), (kappa, 2t + 1), (kappa + 8, ..)
+      const float ks = pow2c(sc & 255), ev = (float)((int)(sc >> 8) - 127);
+      bool over = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] *= qmul[n][e & 1] * ks;
+      if (edge) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = (col0 + 8 * n + 2 * t + (e & 1)) / group, p = p0 + kap + (e >> 1) * 8;
+            if (p >= min(vis(j), cap) || p < low(j)) s[n][e] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) over |= s[n][e] > fminf(ref[n][e & 1] + (8.f - ev), top[n][e & 1] + 60.f);
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float m = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const float r = fmaxf(m + ev, ref[n][e]), f = ex2(ref[n][e] - r);
+            m = fmaxf(m, top[n][e]);
+            l[n][e] *= ex2(top[n][e] - m);
+            ref[n][e] = r;
+            top[n][e] = m;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) o[n][i][e] *= f, o[n][i][e + 2] *= f;
+          }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[n][e] += ex2(s[n][e] - top[n][e]) + ex2(s[n][e + 2] - top[n][e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = ex2(s[n][e] + (ev + 7.f - ref[n][e & 1]));
+        pb[n][0] = movmatrix(pack_f16x2(s[n][0], s[n][1]));
+        pb[n][1] = movmatrix(pack_f16x2(s[n][2], s[n][3]));
+      }
+
+      // O^T += V^T P^T: lane (g, t) reads tokens t, 7 - t, t + 8, 15 - t (kappa of the mma's k = 2t,
+      // 2t + 1, 2t + 8, 2t + 9) of its D / 8 dims; dims 2 i and 2 i + 1 are M tile i's rows g, g + 8
+      uint32_t v[4][D / 32];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = ((r & 1) ? 7 - t : t) + (r >> 1) * 8;
+        if (D == 64) {
+          const uint2 x = lds8(vt + pa_chunk<D>(row, g >> 1) + (g & 1) * 8);
+          v[r][0] = x.x, v[r][1] = x.y;
+        } else {
+#pragma unroll
+          for (int c = 0; c < D / 128; ++c) {
+            const uint4 x = lds16(vt + pa_chunk<D>(row, 8 * c + ((g >> 1) | (g & 1) << 2)));
+            v[r][4 * c] = x.x, v[r][4 * c + 1] = x.y, v[r][4 * c + 2] = x.z, v[r][4 * c + 3] = x.w;
+          }
+        }
+      }
+      auto pv = [&](const uint32_t (&vv)[4][D / 32], float (&acc)[NT][KS][4]) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t a0, a1, a2, a3;
+            const uint32_t sel = h ? 0x7362 : 0x5140;  // (x_2h, y_2h, x_2h+1, y_2h+1)
+            e4m3x4_f16(__byte_perm(vv[0][i], vv[1][i], sel), a0, a1);
+            e4m3x4_f16(__byte_perm(vv[2][i], vv[3][i], sel), a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(acc[n][2 * i + h], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          }
+      };
+      bool row_by_row = false;
+      if (edge) {
+        // tokens that no row of the piece sees hold anything; NaN in one that only some rows see
+        // must not reach the others as 0 NaN
+        bool nan = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int p = p0 + ((r & 1) ? 7 - t : t) + (r >> 1) * 8;
+          const bool seen = p >= any_lo && p < any_hi;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            v[r][i] = seen ? v[r][i] : 0u;
+            nan |= has_nan(v[r][i]);
+          }
+        }
+        row_by_row = __any_sync(0xffffffffu, nan);
+      }
+      if (!row_by_row) {
+        pv(v, o);
+      } else {
+#pragma unroll 1
+        for (int j = j0; j <= j1; ++j) {
+          uint32_t vj[4][D / 32];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int p = p0 + ((r & 1) ? 7 - t : t) + (r >> 1) * 8;
+            const bool seen = p >= low(j) && p < min(vis(j), cap);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) vj[r][i] = seen ? v[r][i] : 0u;
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int c = col0 + 8 * n + 2 * t;
+            const bool mine[2] = {c / group == j, (c + 1) / group == j};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+              uint32_t a0, a1, a2, a3;
+              const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
+              e4m3x4_f16(__byte_perm(vj[0][i / 2], vj[1][i / 2], sel), a0, a1);
+              e4m3x4_f16(__byte_perm(vj[2][i / 2], vj[3][i / 2], sel), a2, a3);
+              float x[4] = {};
+              mma_f16(x, a0, a1, a2, a3, pb[n][0], pb[n][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[n][i][e] += mine[e & 1] ? x[e] : 0.f;
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+
+    // join the warps: the largest reference of each column, then O and l by a tree
+    cp_async_wait<0>();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+    __syncthreads();
+    if (g == 0)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) rl_sm[warp * 8 * NT + 8 * n + 2 * t + e] = make_float4(ref[n][e], top[n][e], l[n][e], 0.f);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float m = -FLT_MAX, c = -FLT_MAX, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float4 x = rl_sm[i * 8 * NT + 8 * n + 2 * t + e];
+          m = fmaxf(m, x.x);
+          c = fmaxf(c, x.y);
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float4 x = rl_sm[i * 8 * NT + 8 * n + 2 * t + e];
+          sum = fmaf(x.z, ex2(x.y - c), sum);
+        }
+        const float f = ex2(ref[n][e] - m);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) o[n][i][e] *= f, o[n][i][e + 2] *= f;
+        ref[n][e] = m;
+        top[n][e] = c;
+        l[n][e] = sum;
+      }
+    float4* mb = reinterpret_cast<float4*>(pa_smem);
+#pragma unroll
+    for (int half = W / 2; half >= 1; half >>= 1) {
+      if (warp >= half && warp < 2 * half)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+            mb[(((warp - half) * NT + n) * KS + i) * 32 + lane] =
+                make_float4(o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]);
+      __syncthreads();
+      if (warp < half)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            const float4 x = mb[((warp * NT + n) * KS + i) * 32 + lane];
+            o[n][i][0] += x.x, o[n][i][1] += x.y, o[n][i][2] += x.z, o[n][i][3] += x.w;
+          }
+      __syncthreads();
+    }
+    const bool whole = step0 == 0 && step1 == w.steps;
+    const int slot = 2 * blockIdx.x + (u == sh.first ? 0 : 1);
+    if (warp == 0)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = 8 * n + 2 * t + e, col = col0 + c;
+          if (col >= w.cols) continue;
+          const int j = col / group, h = hk * group + col % group;
+          // this lane's dims: D / 8 from d0 on (D = 256: two runs of 16, 128 apart)
+          const int d0 = D == 64 ? 8 * g : 16 * ((g >> 1) | (g & 1) << 2);
+          if (whole) {
+            float sum = l[n][e];
+            if (a.sink) sum += ex2(a.sink[h] * 1.44269504f - top[n][e]);
+            const float f = pa_factor(ref[n][e], top[n][e], sum);
+            T* y = reinterpret_cast<T*>(a.out) + (w.row0 + j) * a.out_ld + h * D;
+#pragma unroll
+            for (int i = 0; i < KS / 4; ++i) {
+              float x[8];
+#pragma unroll
+              for (int b = 0; b < 8; ++b) x[b] = o[n][4 * i + b / 2][e + 2 * (b & 1)] * f;
+              *reinterpret_cast<uint4*>(y + (i / 2) * 128 + d0 + (i & 1) * 8) = pack8<F16>(x);
+            }
+          } else {
+            if (g == 0) a.part_rl[(int64_t)slot * 8 * NT + c] = make_float4(ref[n][e], top[n][e], l[n][e], 0.f);
+            float* y = a.part + ((int64_t)slot * 8 * NT + c) * D;
+#pragma unroll
+            for (int i = 0; i < KS / 2; ++i) {
+              const float4 x = make_float4(o[n][2 * i][e], o[n][2 * i][e + 2], o[n][2 * i + 1][e], o[n][2 * i + 1][e + 2]);
+              *reinterpret_cast<float4*>(y + (i / 4) * 128 + d0 + (i & 3) * 4) = x;
+            }
+          }
+        }
+    u += step1 - step0;
+  }
+}
+
+// Join the pieces of the item that begins in share blockIdx.x and goes on past its end (at most one),
+// in the order of the shares. Thread = (column, 4 dims) in turn.
+template <bool F16, int D, int NT>
+__global__ void __launch_bounds__(32 * kPaWarps) paged_join_kernel(const PagedAttnArgs a) {
+  using T = typename Act<F16>::T;
+  __shared__ long long plan_sm[kPaWarps + 2];
+  pdl_wait();
+  const int c = blockIdx.x, kvh = a.cache.kv_heads, group = a.heads / kvh;
+  Share sh = find_share<NT>(a, c, gridDim.x, plan_sm);
+  if (sh.seq < 0) return;
+  int seq = sh.seq;
+  SeqWork w = seq_work<NT>(a, seq);
+  long long seq0 = sh.seq0;
+  while (sh.last > seq0 + w.units) {
+    seq0 += w.units;
+    w = seq_work<NT>(a, ++seq);
+  }
+  const int item = (int)((sh.last - 1 - seq0) / w.steps);
+  const long long u0 = seq0 + (long long)item * w.steps, u1 = u0 + w.steps;
+  if (u0 < sh.first || u1 <= sh.last) return;
+  const int pieces = (int)((u1 - 1) / sh.per) - c + 1;
+  const int ct = item % w.cts, hk = item / w.cts, col0 = ct * 8 * NT;
+  auto slot = [&](int i) { return (int64_t)2 * (c + i) + (i == 0 && u0 != sh.first ? 1 : 0); };
+  for (int x = threadIdx.x; x < 8 * NT * (D / 4); x += blockDim.x) {
+    const int cc = x / (D / 4), d = x % (D / 4) * 4, col = col0 + cc;
+    if (col >= w.cols) break;
+    float m = -FLT_MAX, top = -FLT_MAX, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+      const float4 rl = a.part_rl[slot(i) * 8 * NT + cc];
+      m = fmaxf(m, rl.x);
+      top = fmaxf(top, rl.y);
+    }
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+      const float4 rl = a.part_rl[slot(i) * 8 * NT + cc];
+      const float4 y = *reinterpret_cast<const float4*>(a.part + (slot(i) * 8 * NT + cc) * D + d);
+      const float f = ex2(rl.x - m);
+      sum = fmaf(rl.z, ex2(rl.y - top), sum);
+      o.x = fmaf(y.x, f, o.x), o.y = fmaf(y.y, f, o.y), o.z = fmaf(y.z, f, o.z), o.w = fmaf(y.w, f, o.w);
+    }
+    const int h = hk * group + col % group;
+    if (a.sink) sum += ex2(a.sink[h] * 1.44269504f - top);
+    const float f = pa_factor(m, top, sum);
+    T* y = reinterpret_cast<T*>(a.out) + (w.row0 + col / group) * a.out_ld + h * D + d;
+    *reinterpret_cast<uint2*>(y) = make_uint2(Act<F16>::pack(o.x * f, o.y * f), Act<F16>::pack(o.z * f, o.w * f));
+  }
 }
 
 }  // namespace dsv41
