@@ -17,6 +17,9 @@ using namespace dsv41;
 
 namespace {
 
+// Bytes of x that a CTA of the 4-bit GEMV keeps in shared memory; more is read through L1.
+constexpr int64_t kW4XBytes = 40 * 1024;
+
 template <class T>
 T* ptr(int64_t v) {
   return reinterpret_cast<T*>(v);
@@ -147,16 +150,54 @@ bool w4_ok(const Dsv41GemvW4Args* a) {
          a->x_ld >= a->K && a->y_ld >= a->N && (a->f16 == 0 || a->f16 == 1);
 }
 
+template <int NT, int R, int GS>
+int w4_run(int64_t f16, GemvW4Args g, void* stream) {
+  using P = W4Shape<NT, R, GS>;
+  // a lane's scales of a chunk in one load
+  constexpr int el = P::kEntries > 1 ? P::kEntries / 2 : 1;
+  g.vec = g.group == 32 * GS && g.K / g.group % el == 0 && g.K % kW4Chunk == 0 &&
+          reinterpret_cast<uintptr_t>(g.scales) % (2 * el) == 0 && reinterpret_cast<uintptr_t>(g.zeros) % el == 0;
+  const int64_t x_bytes = (int64_t)g.M * g.K * 2;
+  const bool xs = x_bytes <= kW4XBytes;
+  const int smem = P::kBytes + (xs ? (int)x_bytes : 0);
+  // persistent: as many CTAs as fit, each taking every grid-th row tile
+  const int fit = std::min(std::max(1, 226 * 1024 / (smem + 1024)), 4);
+  const dim3 grid(std::min(cdiv(g.N, P::kRows), device_sms() * fit)), block(32 * kW4Warps);
+  if (xs)
+    return f16 ? launch(gemv_w4_kernel<true, NT, R, GS, true>, grid, block, smem, stream, g)
+               : launch(gemv_w4_kernel<false, NT, R, GS, true>, grid, block, smem, stream, g);
+  return f16 ? launch(gemv_w4_kernel<true, NT, R, GS, false>, grid, block, smem, stream, g)
+             : launch(gemv_w4_kernel<false, NT, R, GS, false>, grid, block, smem, stream, g);
+}
+
+template <int NT, int R>
+int w4_group(int64_t f16, const GemvW4Args& g, void* stream) {
+  const int steps = g.group / 32;
+  return steps % 8 == 0   ? w4_run<NT, R, 8>(f16, g, stream)
+         : steps % 4 == 0 ? w4_run<NT, R, 4>(f16, g, stream)
+         : steps % 2 == 0 ? w4_run<NT, R, 2>(f16, g, stream)
+                          : w4_run<NT, R, 1>(f16, g, stream);
+}
+
 }  // namespace
 
 extern "C" {
 
 int dsv41_gemv_w4(const Dsv41GemvW4Args* a, void* stream) {
   if (!w4_ok(a)) return DSV41_EINVAL;
-  const GemvW4Args g = {ptr<const uint8_t>(a->w), ptr<const void>(a->scales), ptr<const uint8_t>(a->zeros),
-                        ptr<const void>(a->x), ptr<void>(a->y), (int)a->M, (int)a->N, (int)a->K, (int)a->group,
-                        a->x_ld, a->y_ld};
-  return launch(a->f16 ? gemv_w4_kernel<true> : gemv_w4_kernel<false>, dim3(cdiv(g.N, 8)), dim3(256), 0, stream, g);
+  GemvW4Args g = {ptr<const uint8_t>(a->w), ptr<const void>(a->scales), ptr<const uint8_t>(a->zeros),
+                  ptr<const void>(a->x), ptr<void>(a->y), (int)a->M, (int)a->N, (int)a->K, (int)a->group,
+                  a->x_ld, a->y_ld, 0};
+  switch (cdiv(g.M, 8)) {
+    // 32 weight rows a warp share a fragment of x; 16 make more work items of a small matrix (one row,
+    // K 4096: N 4096 5.4 us with 16 and 5.6 with 32; N 8192 8.2 and 7.7; N 129280 79 and 69)
+    case 1: return g.N >= 8192 ? w4_group<1, 2>(a->f16, g, stream) : w4_group<1, 1>(a->f16, g, stream);
+    case 2: return w4_group<2, 2>(a->f16, g, stream);
+    case 3: return w4_group<3, 2>(a->f16, g, stream);
+    case 4: return w4_group<4, 2>(a->f16, g, stream);
+    case 5: return w4_group<5, 2>(a->f16, g, stream);
+    default: return w4_group<6, 2>(a->f16, g, stream);
+  }
 }
 
 int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
