@@ -316,7 +316,9 @@ int dsv41_argmax_decode(const Dsv41ArgmaxArgs* a, void* stream);
 typedef struct {
   int64_t w, scales, zeros, x, y;     /* device pointers */
   int64_t M, N, K, group, x_ld, y_ld, f16;
+  int64_t scratch, scratch_bytes;     /* caller-owned device scratch */
 } Dsv41GemvW4Args;
+int64_t dsv41_gemv_w4_scratch_bytes(const Dsv41GemvW4Args* a);
 int dsv41_gemv_w4(const Dsv41GemvW4Args* a, void* stream);
 
 /* ---------------------------------------------------------------- Paged 8-bit KV cache

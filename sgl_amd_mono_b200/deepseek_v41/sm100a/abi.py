@@ -81,7 +81,7 @@ LmHeadArgs = struct("Dsv41LmHeadArgs", ["M", "V", "K", "vbase", "w", "x", "logit
 ArgmaxArgs = struct("Dsv41ArgmaxArgs", ["M", "best", "ids", "vals", "draft", "per_req", "accept", "next_tok"])
 
 GemvW4Args = struct("Dsv41GemvW4Args", [
-    "w", "scales", "zeros", "x", "y", "M", "N", "K", "group", "x_ld", "y_ld", "f16",
+    "w", "scales", "zeros", "x", "y", "M", "N", "K", "group", "x_ld", "y_ld", "f16", "scratch", "scratch_bytes",
 ])
 
 KvAppendArgs = struct("Dsv41KvAppendArgs", [

@@ -823,6 +823,9 @@ int k2_run(const Dsv41K2Args* a, cudaStream_t st, bool go, int64_t* need) {
 void dsv41::count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 int dsv41::device_sms() { return sm_count(); }
 bool dsv41::pdl_on() { return use_pdl(); }
+bool dsv41::byte_tile_map(CUtensorMap* m, const void* w, int rows, int row_bytes) {
+  return dense_weight_map(m, w, rows, row_bytes);
+}
 
 extern "C" {
 
@@ -831,6 +834,7 @@ int64_t dsv41_launch_count(void) { return g_launches.load(); }
 int dsv41_device_error(void) {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, dsv41::g_tc_error, sizeof(v)) != cudaSuccess) return launch_status();
+  if (!v && !gqa_device_error(&v)) return launch_status();
   return v ? DSV41_EDEVICE : DSV41_OK;
 }
 

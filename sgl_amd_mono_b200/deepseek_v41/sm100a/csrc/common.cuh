@@ -6,6 +6,7 @@
 // CPU oracle bit for bit where a stage's output must be bit-exact (KV records, routing).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -297,5 +298,10 @@ cudaError_t ensure_smem(const void* kernel, int bytes);
 void count_launch();
 int device_sms();
 bool pdl_on();
+// The tensor map of a byte matrix [rows, row_bytes] read in 256-row x 128-byte boxes with the 128-byte
+// swizzle, zeros past its ends; row_bytes a multiple of 16.
+bool byte_tile_map(CUtensorMap* m, const void* w, int rows, int row_bytes);
+// The error word of the grouped-query kernels' bounded waits; false when it cannot be read.
+bool gqa_device_error(int* v);
 
 }  // namespace dsv41

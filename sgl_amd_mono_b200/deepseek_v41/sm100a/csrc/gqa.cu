@@ -1,55 +1,18 @@
-// extern "C" entry points of the grouped-query decode operators (include/dsv41_b200.h): the 4-bit
-// GEMV, the paged 8-bit cache's append and the attention over it. Argument checks, then the launches
-// on the caller's stream.
-#include <algorithm>
+// extern "C" entry points of the paged 8-bit cache's append and the attention over it
+// (include/dsv41_b200.h): argument checks, then the launches on the caller's stream.
 #include <climits>
-#include <cstdio>
 #include <cstring>
 #include <type_traits>
 
 #include "../../../../include/dsv41_b200.h"
-#include "gemv_w4.cuh"
 #include "gqa.cuh"
+#include "gqa_launch.cuh"
 #include "kv_append.cuh"
 #include "paged_attn.cuh"
 
 using namespace dsv41;
 
 namespace {
-
-// Bytes of x that a CTA of the 4-bit GEMV keeps in shared memory; more is read through L1.
-constexpr int64_t kW4XBytes = 40 * 1024;
-
-template <class T>
-T* ptr(int64_t v) {
-  return reinterpret_cast<T*>(v);
-}
-
-// One launch with programmatic dependent launch (every kernel waits before it reads).
-template <class Args>
-int launch(void (*kernel)(const Args), dim3 grid, dim3 block, int smem, void* stream, const Args& args) {
-  cudaError_t e = smem > 48 * 1024 ? ensure_smem(reinterpret_cast<const void*>(kernel), smem) : cudaSuccess;
-  if (e == cudaSuccess) {
-    count_launch();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = pdl_on() ? 1 : 0;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, args);
-  }
-  if (e == cudaSuccess) return DSV41_OK;
-  cudaGetLastError();
-  fprintf(stderr, "dsv41: launch failed: %s\n", cudaGetErrorString(e));
-  return DSV41_ELAUNCH;
-}
-
-int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Rows [T, heads, dim] of 2-byte values, ld elements apart.
 bool rows_ok(int64_t p, int64_t ld, int64_t heads, int64_t dim) {
@@ -143,62 +106,9 @@ int attn_run(const Dsv41PagedAttnArgs* a, void* stream) {
   return rc ? rc : launch(paged_join_kernel<F16, D, NT>, dim3((unsigned)ctas), dim3(32 * kPaWarps), 0, stream, p);
 }
 
-bool w4_ok(const Dsv41GemvW4Args* a) {
-  return a && a->w && a->w % 16 == 0 && a->scales && a->scales % 2 == 0 && a->x && a->x % 16 == 0 && a->y &&
-         a->y % 2 == 0 && a->M >= 1 && a->M <= kW4MaxRows && a->N >= 1 && a->N <= (1 << 24) && a->group >= 32 &&
-         a->group % 32 == 0 && a->K >= a->group && a->K <= (1 << 24) && a->K % a->group == 0 && a->x_ld % 8 == 0 &&
-         a->x_ld >= a->K && a->y_ld >= a->N && (a->f16 == 0 || a->f16 == 1);
-}
-
-template <int NT, int R, int GS>
-int w4_run(int64_t f16, GemvW4Args g, void* stream) {
-  using P = W4Shape<NT, R, GS>;
-  // a lane's scales of a chunk in one load
-  constexpr int el = P::kEntries > 1 ? P::kEntries / 2 : 1;
-  g.vec = g.group == 32 * GS && g.K / g.group % el == 0 && g.K % kW4Chunk == 0 &&
-          reinterpret_cast<uintptr_t>(g.scales) % (2 * el) == 0 && reinterpret_cast<uintptr_t>(g.zeros) % el == 0;
-  const int64_t x_bytes = (int64_t)g.M * g.K * 2;
-  const bool xs = x_bytes <= kW4XBytes;
-  const int smem = P::kBytes + (xs ? (int)x_bytes : 0);
-  // persistent: as many CTAs as fit, each taking every grid-th row tile
-  const int fit = std::min(std::max(1, 226 * 1024 / (smem + 1024)), 4);
-  const dim3 grid(std::min(cdiv(g.N, P::kRows), device_sms() * fit)), block(32 * kW4Warps);
-  if (xs)
-    return f16 ? launch(gemv_w4_kernel<true, NT, R, GS, true>, grid, block, smem, stream, g)
-               : launch(gemv_w4_kernel<false, NT, R, GS, true>, grid, block, smem, stream, g);
-  return f16 ? launch(gemv_w4_kernel<true, NT, R, GS, false>, grid, block, smem, stream, g)
-             : launch(gemv_w4_kernel<false, NT, R, GS, false>, grid, block, smem, stream, g);
-}
-
-template <int NT, int R>
-int w4_group(int64_t f16, const GemvW4Args& g, void* stream) {
-  const int steps = g.group / 32;
-  return steps % 8 == 0   ? w4_run<NT, R, 8>(f16, g, stream)
-         : steps % 4 == 0 ? w4_run<NT, R, 4>(f16, g, stream)
-         : steps % 2 == 0 ? w4_run<NT, R, 2>(f16, g, stream)
-                          : w4_run<NT, R, 1>(f16, g, stream);
-}
-
 }  // namespace
 
 extern "C" {
-
-int dsv41_gemv_w4(const Dsv41GemvW4Args* a, void* stream) {
-  if (!w4_ok(a)) return DSV41_EINVAL;
-  GemvW4Args g = {ptr<const uint8_t>(a->w), ptr<const void>(a->scales), ptr<const uint8_t>(a->zeros),
-                  ptr<const void>(a->x), ptr<void>(a->y), (int)a->M, (int)a->N, (int)a->K, (int)a->group,
-                  a->x_ld, a->y_ld, 0};
-  switch (cdiv(g.M, 8)) {
-    // 32 weight rows a warp share a fragment of x; 16 make more work items of a small matrix (one row,
-    // K 4096: N 4096 5.4 us with 16 and 5.6 with 32; N 8192 8.2 and 7.7; N 129280 79 and 69)
-    case 1: return g.N >= 8192 ? w4_group<1, 2>(a->f16, g, stream) : w4_group<1, 1>(a->f16, g, stream);
-    case 2: return w4_group<2, 2>(a->f16, g, stream);
-    case 3: return w4_group<3, 2>(a->f16, g, stream);
-    case 4: return w4_group<4, 2>(a->f16, g, stream);
-    case 5: return w4_group<5, 2>(a->f16, g, stream);
-    default: return w4_group<6, 2>(a->f16, g, stream);
-  }
-}
 
 int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
   if (!append_ok(a)) return DSV41_EINVAL;

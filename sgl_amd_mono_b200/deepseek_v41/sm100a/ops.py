@@ -69,5 +69,9 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch
         raise RuntimeError(f"gemv_w4: out {tuple(out.shape)} {out.dtype} on {out.device}: want [{M}, {N}] {x.dtype}")
     a = abi.GemvW4Args(w=_ptr(w), scales=_ptr(scales), zeros=0 if zeros is None else _ptr(zeros), x=_ptr(x),
                        y=_ptr(out), M=M, N=N, K=K, group=K // groups, x_ld=x_ld, y_ld=y_ld, f16=x.dtype is torch.float16)
+    need = ext.query("dsv41_gemv_w4_scratch_bytes", a)
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.scratch, a.scratch_bytes = _ptr(scratch), need
     ext.call("dsv41_gemv_w4", a, _stream())
     return out

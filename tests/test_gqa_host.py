@@ -21,7 +21,7 @@ def _call(fn, a):
 # Valid but for one field each: an invalid argument is refused before anything is launched, so the
 # pointers are never followed.
 P = 1 << 20
-W4 = dict(w=P, scales=P, zeros=0, x=P, y=P, M=4, N=64, K=256, group=64, x_ld=256, y_ld=64, f16=0)
+W4 = dict(w=P, scales=P, zeros=0, x=P, y=P, M=4, N=64, K=256, group=64, x_ld=256, y_ld=64, f16=0, scratch=P, scratch_bytes=1 << 40)
 PAGED = dict(T=4, seqs=2, heads=8, kv_heads=2, dim=64, f16=0, cu_rows=P, lens=P, table=P, table_ld=4, width=4,
              k_cache=P, v_cache=P, k_codes=P, v_codes=P, pages=9, page=32, block=16, q=P, q_ld=512)
 APPEND = dict(PAGED, rope=32, neox=1, q_out=P, q_out_ld=512, k=P, k_ld=128, v=P, v_ld=128, cos_sin=P, rope_rows=10)
@@ -47,7 +47,11 @@ BAD_ATTN = [dict(q=0), dict(out=0), dict(out=P + 2), dict(out_ld=504), dict(wind
 @pytest.mark.parametrize("bad", BAD_W4, ids=str)
 def test_gemv_w4_refuses(bad):
     from sgl_amd_mono_b200.deepseek_v41.sm100a import abi
-    assert _call("dsv41_gemv_w4", abi.GemvW4Args(**{**W4, **bad})) == EINVAL
+    from sgl_amd_mono_b200.common import ext
+    a = abi.GemvW4Args(**{**W4, **bad})
+    assert _call("dsv41_gemv_w4", a) == EINVAL
+    with pytest.raises(ext.ExtError):
+        ext.query("dsv41_gemv_w4_scratch_bytes", a)
 
 
 @pytest.mark.parametrize("bad", BAD_PAGED + BAD_APPEND, ids=str)
@@ -64,6 +68,17 @@ def test_paged_attn_refuses(bad):
     assert _call("dsv41_paged_attn", a) == EINVAL
     with pytest.raises(ext.ExtError):
         ext.query("dsv41_paged_attn_scratch_bytes", a)
+
+
+@pytest.mark.parametrize("short", [dict(scratch=0), dict(scratch=P + 8), dict(scratch_bytes=-1)], ids=str)
+def test_scratch_that_does_not_do_is_refused(short):
+    from sgl_amd_mono_b200.common import ext
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import abi
+    a = abi.PagedAttnArgs(**{**ATTN, **short})
+    assert _call("dsv41_paged_attn", a) == -3
+    big = {**W4, "M": 48, "N": 8192, "K": 4096, "x_ld": 4096, "y_ld": 8192}
+    assert ext.query("dsv41_gemv_w4_scratch_bytes", abi.GemvW4Args(**big)) > 0
+    assert _call("dsv41_gemv_w4", abi.GemvW4Args(**{**big, **short})) == -3
 
 
 def test_null_arguments_are_refused():
