@@ -113,18 +113,27 @@ extern "C" {
 int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
   if (!append_ok(a)) return DSV41_EINVAL;
   if (!a->T || !a->seqs) return DSV41_OK;
-  const KvAppendArgs k = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->rope, (int)a->neox,
-                          ptr<const void>(a->q), ptr<const void>(a->k), ptr<const void>(a->v), ptr<void>(a->q_out),
-                          a->q_ld, a->q_out_ld, a->k_ld, a->v_ld, ptr<const float>(a->cos_sin), a->rope_rows};
-  const int items = (a->q ? k.heads : 0) + 2 * k.cache.kv_heads;
-  const dim3 grid(k.rows.T, cdiv(items, 4));
+  KvAppendArgs k = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->rope, (int)a->neox,
+                    ptr<const void>(a->q), ptr<const void>(a->k), ptr<const void>(a->v), ptr<void>(a->q_out),
+                    a->q_ld, a->q_out_ld, a->k_ld, a->v_ld, ptr<const float>(a->cos_sin), a->rope_rows};
+  // A warp looks through one row where most rows begin a block of their own (decode and verify rows),
+  // else through 16, so that a prompt's warps nearly all find one block. A thread takes one query head
+  // while the rows are too few to fill the GPU, else four, for which it reads the angles once.
+  k.window = a->T >= 8 * a->seqs ? 16 : 1;
+  k.head_step = a->T * a->heads * a->dim / 16 < 148 * 2048 ? 1 : 4;
+  const int64_t warps = cdiv64(a->T, k.window) * 2 * a->kv_heads;
+  const int64_t q_threads = a->q ? a->T * cdiv64(a->heads, k.head_step) * (a->dim / 16) : 0;
+  const int64_t kv_ctas = cdiv64(warps, kApThreads / 32), ctas = kv_ctas + cdiv64(q_threads, kApThreads);
+  if (ctas > INT_MAX) return DSV41_EINVAL;
+  k.kv_ctas = (int)kv_ctas;
+  const dim3 grid((unsigned)ctas), cta(kApThreads);
   switch (a->dim * 2 + a->f16) {
-    case 128: return launch(kv_append_kernel<false, 64>, grid, dim3(128), 0, stream, k);
-    case 129: return launch(kv_append_kernel<true, 64>, grid, dim3(128), 0, stream, k);
-    case 256: return launch(kv_append_kernel<false, 128>, grid, dim3(128), 0, stream, k);
-    case 257: return launch(kv_append_kernel<true, 128>, grid, dim3(128), 0, stream, k);
-    case 512: return launch(kv_append_kernel<false, 256>, grid, dim3(128), 0, stream, k);
-    default: return launch(kv_append_kernel<true, 256>, grid, dim3(128), 0, stream, k);
+    case 128: return launch(kv_append_kernel<false, 64>, grid, cta, 0, stream, k);
+    case 129: return launch(kv_append_kernel<true, 64>, grid, cta, 0, stream, k);
+    case 256: return launch(kv_append_kernel<false, 128>, grid, cta, 0, stream, k);
+    case 257: return launch(kv_append_kernel<true, 128>, grid, cta, 0, stream, k);
+    case 512: return launch(kv_append_kernel<false, 256>, grid, cta, 0, stream, k);
+    default: return launch(kv_append_kernel<true, 256>, grid, cta, 0, stream, k);
   }
 }
 

@@ -5,11 +5,18 @@
 // code)); when the code grows from c0 to c1, the older bytes become e4m3(byte 2^(c0 - c1)). The
 // scale is a power of two, so only bytes that fall into e4m3's subnormal range change value.
 // A block is written by one warp, that of its first new row, so no two warps meet in a block.
+//
+// The work is copying, so everything moves 16 bytes a lane at a time in units of 16 dims: two 8-dim
+// pieces that hold 8 whole rotation pairs and share 8 angles, side by side for pairs (2j, 2j + 1) and
+// half a rotation apart for (j, j + rope / 2). A block's rows are read twice, for the largest magnitude
+// and to be written; the second time from L1.
 #pragma once
 
 #include "gqa.cuh"
 
 namespace dsv41 {
+
+constexpr int kApThreads = 256;
 
 struct KvAppendArgs {
   StepRows rows;
@@ -20,95 +27,207 @@ struct KvAppendArgs {
   int64_t q_ld, q_out_ld, k_ld, v_ld;
   const float* cos_sin;
   int64_t rope_rows;
+  int window;     // rows a warp looks through for blocks to write
+  int kv_ctas;    // CTAs of the keys and values; the rest rotate queries
+  int head_step;  // heads a query thread takes
 };
 
-// e4m3 byte of x, saturating; NaN stays NaN.
-__device__ __forceinline__ uint8_t kv_byte(float x) {
-  return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+// Dims of unit u of a head: its two pieces of 8, and the first of its 8 angles (< 0: not rotated).
+struct RopeUnit {
+  int d0, d1, angle;
+};
+__device__ __forceinline__ RopeUnit rope_unit(int u, int dim, int rope, int neox) {
+  const int ur = u - (dim - rope) / 16;
+  if (ur >= 0 && neox) return {dim - rope + 8 * ur, dim - rope / 2 + 8 * ur, 8 * ur};
+  return {16 * u, 16 * u + 8, ur >= 0 ? 8 * ur : -1};
 }
 
-// Element d of a row's head, rotated when cs is not null: the pair's two products and their sum are
-// each rounded in fp32, as the cache's contract says.
-template <bool F16, int D>
-__device__ __forceinline__ float rotated(const typename Act<F16>::T* x, int d, const float* cs, int rope, int neox) {
-  const float v = Act<F16>::f(x[d]);
-  const int i = d - (D - rope);
-  if (!cs || i < 0) return v;
-  const int half = rope / 2;
-  const int pr = neox ? (i < half ? i : i - half) : i >> 1;
-  const bool first = neox ? i < half : !(i & 1);
-  const float o = Act<F16>::f(x[neox ? (first ? d + half : d - half) : (d ^ 1)]);
-  const float c = cs[pr], s = cs[half + pr];
-  return first ? __fsub_rn(__fmul_rn(v, c), __fmul_rn(o, s)) : __fadd_rn(__fmul_rn(o, s), __fmul_rn(v, c));
-}
-
-// Grid (T, ceil((heads + 2 kv_heads) / 4)), 128 threads: a warp a (row, head of q, k or v).
-template <bool F16, int D>
-__global__ void __launch_bounds__(128) kv_append_kernel(const KvAppendArgs a) {
-  using T = typename Act<F16>::T;
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int r = blockIdx.x, kvh = a.cache.kv_heads;
-  int h = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (!a.q) h += a.heads;
-  if (h >= a.heads + 2 * kvh) return;
-  const int seq = row_seq(a.rows, r, lane);
-  if (seq < 0) return;
-  const int first = a.rows.cu_rows ? a.rows.cu_rows[seq] : r;
-  const int n = a.rows.cu_rows ? a.rows.cu_rows[seq + 1] - first : 1;
-  const int64_t pos = (int64_t)a.rows.lens[seq] - n + (r - first);
-  auto row_cs = [&](int64_t p) {
-    return a.rope ? a.cos_sin + rope_row(max(p, (int64_t)0), a.rope_rows) * a.rope : nullptr;
-  };
-  if (h < a.heads) {
-    const T* x = reinterpret_cast<const T*>(a.q) + r * a.q_ld + h * D;
-    T* y = reinterpret_cast<T*>(a.q_out) + r * a.q_out_ld + h * D;
-    const float* cs = row_cs(pos);
-    float v[D / 32];
+// (A plain load: the queries may be rotated in place.)
+template <bool F16>
+__device__ __forceinline__ void load8(const typename Act<F16>::T* x, float* v) {
+  const uint4 w = *reinterpret_cast<const uint4*>(x);
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) v[i] = rotated<F16, D>(x, lane + 32 * i, cs, a.rope, a.neox);
-    __syncwarp();  // q_out may be q
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) y[lane + 32 * i] = Act<F16>::r(v[i]);
-    return;
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Act<F16>::unpack(ws[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
   }
-  if (pos < 0 || pos >= (int64_t)a.rows.width * a.cache.page) return;
-  const int block = a.cache.block, in = (int)(pos % block);
-  if (r != first && in != 0) return;  // the warp of the block's first new row writes it
+}
+struct Angles {
+  float c[8], s[8];
+};
+__device__ __forceinline__ void load_angles(const float* row, int rope, int angle, Angles& a) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 c = __ldg(reinterpret_cast<const float4*>(row + angle) + i);
+    const float4 s = __ldg(reinterpret_cast<const float4*>(row + rope / 2 + angle) + i);
+    a.c[4 * i] = c.x, a.c[4 * i + 1] = c.y, a.c[4 * i + 2] = c.z, a.c[4 * i + 3] = c.w;
+    a.s[4 * i] = s.x, a.s[4 * i + 1] = s.y, a.s[4 * i + 2] = s.z, a.s[4 * i + 3] = s.w;
+  }
+}
+// The pair's two products and their sum are each rounded in fp32, as the cache's contract says.
+__device__ __forceinline__ void rotate_pair(float& x, float& y, float c, float s) {
+  const float a = x, b = y;
+  x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+  y = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
+}
+__device__ __forceinline__ void rotate16(float (&v)[16], const Angles& a, int neox) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (neox) rotate_pair(v[i], v[8 + i], a.c[i], a.s[i]);
+    else rotate_pair(v[2 * i], v[2 * i + 1], a.c[i], a.s[i]);
+  }
+}
+// 4 e4m3 bytes, saturating; NaN stays NaN.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+// The rows [r, r + rows) of one head, tokens `pos` .. of one block, by one warp.
+template <bool F16, int D>
+__device__ __forceinline__ void append_block(const KvAppendArgs& a, int seq, int r, int rows, int64_t pos, int item) {
+  using T = typename Act<F16>::T;
+  constexpr int UNITS = D / 16, PER = 32 / UNITS;  // lanes a row, rows at a time
+  const int lane = threadIdx.x & 31, kvh = a.cache.kv_heads, block = a.cache.block, page = a.cache.page;
   const int pg = token_page(a.rows, a.cache, seq, (int)pos);
   if (pg < 0) return;
-  const int off = (int)(pos % a.cache.page);
-  const int rows = min(min(block - in, n - (r - first)), a.rows.T - r);
-  const bool is_k = h < a.heads + kvh;
-  const int hk = h - a.heads - (is_k ? 0 : kvh);
+  const bool is_k = item < kvh;
+  const int hk = is_k ? item : item - kvh;
+  const int in = (int)(pos % block), off = (int)(pos % page) - in;  // the block's first token in its page
   const T* x = reinterpret_cast<const T*>(is_k ? a.k : a.v) + hk * D;
   const int64_t ld = is_k ? a.k_ld : a.v_ld;
-  uint8_t* cache = is_k ? a.cache.k : a.cache.v;
-  uint8_t* codes = is_k ? a.cache.k_codes : a.cache.v_codes;
   const int64_t head = (int64_t)pg * kvh + hk;
-  uint8_t* dst = cache + (head * a.cache.page + off - in) * D;  // the block's first token
-  uint8_t* cp = codes + head * (a.cache.page / block) + off / block;
+  uint8_t* dst = (is_k ? a.cache.k : a.cache.v) + (head * page + off) * D;
+  uint8_t* cp = (is_k ? a.cache.k_codes : a.cache.v_codes) + head * (page / block) + off / block;
+  const int rope = is_k ? a.rope : 0;
+  const RopeUnit ru = rope_unit(lane % UNITS, D, rope, a.neox);
+  const int old = in ? *cp : 0;
+  auto value = [&](int i, float (&v)[16]) {
+    const T* row = x + (r + i) * ld;
+    load8<F16>(row + ru.d0, v);
+    load8<F16>(row + ru.d1, v + 8);
+    if (rope && ru.angle >= 0) {
+      Angles an;
+      load_angles(a.cos_sin + rope_row(pos + i, a.rope_rows) * rope, rope, ru.angle, an);
+      rotate16(v, an, a.neox);
+    }
+  };
   float amax = 0.f;
-  for (int i = 0; i < rows; ++i)
-    for (int d = lane; d < D; d += 32)
-      amax = fmaxf(amax, fabsf(rotated<F16, D>(x + (r + i) * ld, d, is_k ? row_cs(pos + i) : nullptr, a.rope, a.neox)));
+#pragma unroll 2
+  for (int i = lane / UNITS; i < rows; i += PER) {
+    float v[16];
+    value(i, v);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(v[e]));  // NaN does not count
+  }
   amax = fminf(warp_max(amax), 3.402823466e38f);
   int code = code_ceil(__fdiv_rn(fmaxf(amax, 1e-4f), kFp8Max));
   if (in) {
-    const int old = *cp;
-    if (old >= code) code = old;
-    else {
+    if (old >= code) {
+      code = old;
+    } else {
       const float m = pow2c(max(127 + old - code, 0));
-      for (int i = lane; i < in * D; i += 32) dst[i] = kv_byte(e4m3_float(dst[i]) * m);
+      uint32_t* w = reinterpret_cast<uint32_t*>(dst);
+      for (int i = lane; i < in * (D / 4); i += 32) {
+        const uint32_t b = w[i];
+        const float2 lo = e4m3x2_float2(b & 0xffff), hi = e4m3x2_float2(b >> 16);
+        w[i] = e4m3x4(lo.x * m, lo.y * m, hi.x * m, hi.y * m);
+      }
     }
   }
   const float mul = mx_mul(code);
-  for (int i = 0; i < rows; ++i)
-    for (int d = lane; d < D; d += 32)
-      dst[(in + i) * D + d] =
-          kv_byte(rotated<F16, D>(x + (r + i) * ld, d, is_k ? row_cs(pos + i) : nullptr, a.rope, a.neox) * mul);
+#pragma unroll 2
+  for (int i = lane / UNITS; i < rows; i += PER) {
+    float v[16];
+    value(i, v);
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = e4m3x4(v[4 * e] * mul, v[4 * e + 1] * mul, v[4 * e + 2] * mul, v[4 * e + 3] * mul);
+    uint8_t* y = dst + (in + i) * D;
+    *reinterpret_cast<uint2*>(y + ru.d0) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(y + ru.d1) = make_uint2(w[2], w[3]);
+  }
   __syncwarp();
   if (lane == 0) *cp = (uint8_t)code;
+}
+
+// The sequence of row r by binary search, or -1 for a row behind the last sequence.
+__device__ __forceinline__ int row_seq_search(const StepRows& s, int r) {
+  if (!s.cu_rows) return r;
+  int lo = 0, hi = s.seqs;  // the first sequence whose end is past r
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (__ldg(s.cu_rows + mid + 1) > r) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo < s.seqs && __ldg(s.cu_rows + lo) <= r ? lo : -1;
+}
+
+// CTAs [0, kv_ctas): a warp a (window of rows, key or value head); the others: a thread a (row, head_step
+// query heads, unit).
+template <bool F16, int D>
+__global__ void __launch_bounds__(kApThreads) kv_append_kernel(const KvAppendArgs a) {
+  using T = typename Act<F16>::T;
+  constexpr int UNITS = D / 16;
+  pdl_wait();
+  const StepRows& st = a.rows;
+  if ((int)blockIdx.x < a.kv_ctas) {
+    const int lane = threadIdx.x & 31, items = 2 * a.cache.kv_heads, block = a.cache.block;
+    const int64_t wi = (int64_t)blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5);
+    const int64_t w0 = wi / items * a.window;
+    if (w0 >= st.T) return;
+    const int item = (int)(wi % items), w1 = (int)min(w0 + a.window, (int64_t)st.T);
+    const int64_t cap = (int64_t)st.width * a.cache.page;
+    int r = (int)w0, seq = row_seq(st, r, lane);
+    while (r < w1 && seq >= 0 && seq < st.seqs) {
+      const int first = st.cu_rows ? st.cu_rows[seq] : seq, end = st.cu_rows ? st.cu_rows[seq + 1] : seq + 1;
+      if (end <= r) {
+        ++seq;
+        continue;
+      }
+      const int64_t pos = (int64_t)st.lens[seq] - end + r;
+      int rows = end - r;  // to the next block's first row, or the sequence's end
+      if (pos < 0) {
+        rows = (int)min((int64_t)rows, -pos);
+      } else {
+        rows = min(min(rows, block - (int)(pos % block)), st.T - r);
+        // the block's first new row leads: the sequence's first, one at the block's start, or token 0
+        if ((r == first || pos % block == 0) && pos < cap) append_block<F16, D>(a, seq, r, rows, pos, item);
+      }
+      r += rows;
+    }
+    return;
+  }
+  const int groups = (a.heads + a.head_step - 1) / a.head_step;
+  const int64_t ti = (int64_t)(blockIdx.x - a.kv_ctas) * kApThreads + threadIdx.x;
+  const int64_t row = ti / (groups * UNITS);
+  if (row >= st.T) return;
+  const int r = (int)row, u = (int)(ti % UNITS), h0 = (int)(ti / UNITS % groups) * a.head_step;
+  const int seq = row_seq_search(st, r);
+  if (seq < 0) return;
+  const RopeUnit ru = rope_unit(u, D, a.rope, a.neox);
+  Angles an;
+  if (a.rope && ru.angle >= 0) {
+    const int64_t pos = (int64_t)st.lens[seq] - (st.cu_rows ? st.cu_rows[seq + 1] : seq + 1) + r;
+    load_angles(a.cos_sin + rope_row(max(pos, (int64_t)0), a.rope_rows) * a.rope, a.rope, ru.angle, an);
+  }
+  const T* x = reinterpret_cast<const T*>(a.q) + row * a.q_ld;
+  T* y = reinterpret_cast<T*>(a.q_out) + row * a.q_out_ld;
+  const int h1 = min(h0 + a.head_step, a.heads);
+#pragma unroll 4
+  for (int h = h0; h < h1; ++h) {
+    float v[16];
+    load8<F16>(x + h * D + ru.d0, v);
+    load8<F16>(x + h * D + ru.d1, v + 8);
+    if (a.rope && ru.angle >= 0) rotate16(v, an, a.neox);
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = Act<F16>::pack(v[2 * e], v[2 * e + 1]);
+    *reinterpret_cast<uint4*>(y + h * D + ru.d0) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(y + h * D + ru.d1) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
 }
 
 }  // namespace dsv41
