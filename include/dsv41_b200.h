@@ -312,7 +312,8 @@ int dsv41_argmax_decode(const Dsv41ArgmaxArgs* a, void* stream);
  * k in the low nibble) and read in place; scales [N, K / group] of x's type; zeros u8
  * [N, K / group] (values 0 .. 15) or 0 for 8 everywhere; x [M, x_ld] and y [M, y_ld] bf16, or f16
  * with f16 = 1. M <= 48, K a multiple of group, group a multiple of 32; w and x 16-byte aligned,
- * x_ld a multiple of 8. No counterpart in the reference (its dense projections are FP8). */
+ * x_ld a multiple of 8. Up to 16 rows need no scratch. No counterpart in the reference (its dense
+ * projections are FP8). */
 typedef struct {
   int64_t w, scales, zeros, x, y;     /* device pointers */
   int64_t M, N, K, group, x_ld, y_ld, f16;

@@ -46,19 +46,31 @@ def check(rc: int, what: str) -> int:
     return rc
 
 
+_calls: dict = {}    # launch entry points with their prototypes set, by name
+_queries: dict = {}
+
+
 def call(fn: str, args: ctypes.Structure, stream: int) -> None:
     """``fn(&args, stream)``, raising on a negative status."""
-    f = getattr(lib(), fn)
-    f.restype = ctypes.c_int
-    f.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
-    check(f(ctypes.byref(args), ctypes.c_void_p(stream)), fn)
+    f = _calls.get(fn)
+    if f is None:
+        f = getattr(lib(), fn)
+        f.restype = ctypes.c_int
+        f.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        _calls[fn] = f
+    rc = f(ctypes.byref(args), stream)
+    if rc < 0:
+        check(rc, fn)
 
 
 def query(fn: str, args: ctypes.Structure) -> int:
     """An int64 query ``fn(&args)`` (scratch sizes), raising on a negative status."""
-    f = getattr(lib(), fn)
-    f.restype = ctypes.c_int64
-    f.argtypes = [ctypes.c_void_p]
+    f = _queries.get(fn)
+    if f is None:
+        f = getattr(lib(), fn)
+        f.restype = ctypes.c_int64
+        f.argtypes = [ctypes.c_void_p]
+        _queries[fn] = f
     return check(int(f(ctypes.byref(args))), fn)
 
 

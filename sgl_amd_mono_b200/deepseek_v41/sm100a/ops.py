@@ -6,7 +6,7 @@ import torch
 
 from ...common import ext
 from . import abi
-from .paged import check_device
+from .paged import current_stream
 
 W4_MAX_ROWS = 48  # of gemv_w4
 
@@ -40,38 +40,46 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch
     without them), times ``scales`` ([N, K / group] of x's type); group a multiple of 32."""
     if x.dim() != 2 or w.dim() != 2 or scales.dim() != 2:
         raise RuntimeError(f"gemv_w4: x {tuple(x.shape)}, w {tuple(w.shape)}, scales {tuple(scales.shape)}: want matrices")
-    (M, K), N, groups = x.shape, w.shape[0], scales.shape[1]
-    dev = x.device
-    check_device(dev, "gemv_w4")
-    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
-        raise RuntimeError(f"gemv_w4: x of {x.dtype}, want bfloat16 or float16")
+    dev, dtype = x.get_device(), x.dtype
+    stream = current_stream(dev, "gemv_w4")
+    (M, K), (N, groups), x_at, w_at = x.shape, scales.shape, x.data_ptr(), w.data_ptr()
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise RuntimeError(f"gemv_w4: x of {dtype}, want bfloat16 or float16")
     if not 1 <= M <= W4_MAX_ROWS or not N or not groups or K % groups or K // groups % 32:
         raise RuntimeError(f"gemv_w4: {M} rows of {K} in {groups} groups, {N} outputs: at most {W4_MAX_ROWS} rows, groups "
                            "a multiple of 32")
-    if w.shape[1] * 2 != K or w.dtype != torch.uint8 or w.device != dev or not w.is_contiguous() or w.data_ptr() % 16:
+    if w.shape != (N, K // 2) or w.dtype is not torch.uint8 or w.get_device() != dev or not w.is_contiguous() or w_at & 15:
         raise RuntimeError(f"gemv_w4: w {tuple(w.shape)} {w.dtype} on {w.device}: want contiguous, 16-byte aligned "
-                           f"[{N}, {K // 2}] uint8 on {dev}")
-    if scales.shape[0] != N or scales.dtype != x.dtype or scales.device != dev or not scales.is_contiguous():
-        raise RuntimeError(f"gemv_w4: scales {tuple(scales.shape)} {scales.dtype} on {scales.device}: want [{N}, groups] "
-                           f"{x.dtype} on {dev}")
-    if zeros is not None and (zeros.shape != scales.shape or zeros.dtype != torch.uint8 or zeros.device != dev
-                              or not zeros.is_contiguous()):
-        raise RuntimeError(f"gemv_w4: zeros {tuple(zeros.shape)} {zeros.dtype} on {zeros.device}: want [{N}, {groups}] "
-                           f"uint8 on {dev}")
-    x_ld = x.stride(0) if M > 1 else -(-max(x.stride(0), K) // 8) * 8
-    if x.stride(1) != 1 or x_ld % 8 or x_ld < K or _ptr(x) % 16:
-        raise RuntimeError(f"gemv_w4: x strides {x.stride()} at {_ptr(x):#x}: want contiguous rows a multiple of 8 values "
+                           f"[{N}, {K // 2}] uint8 on {x.device}")
+    if scales.dtype is not dtype or scales.get_device() != dev or not scales.is_contiguous():
+        raise RuntimeError(f"gemv_w4: scales of {scales.dtype} on {scales.device}: want contiguous {dtype} on {x.device}")
+    x_ld, one = x.stride()
+    if M < 2:
+        x_ld = K
+    if one != 1 or x_ld & 7 or x_ld < K or x_at & 15:
+        raise RuntimeError(f"gemv_w4: x strides {x.stride()} at {x_at:#x}: want contiguous rows a multiple of 8 values "
                            "apart, 16-byte aligned")
+    a = abi.GemvW4Args(w_at, scales.data_ptr(), 0, x_at, 0, M, N, K, K // groups, x_ld, N, dtype is torch.float16)
+    if zeros is not None:
+        if zeros.shape != (N, groups) or zeros.dtype is not torch.uint8 or zeros.get_device() != dev \
+                or not zeros.is_contiguous():
+            raise RuntimeError(f"gemv_w4: zeros {tuple(zeros.shape)} {zeros.dtype} on {zeros.device}: want [{N}, {groups}] "
+                               f"uint8 on {x.device}")
+        a.zeros = zeros.data_ptr()
     if out is None:
-        out = torch.empty(M, N, dtype=x.dtype, device=dev)
-    y_ld = out.stride(0) if M > 1 else N
-    if out.shape != (M, N) or out.dtype != x.dtype or out.device != dev or (N > 1 and out.stride(1) != 1) or y_ld < N:
-        raise RuntimeError(f"gemv_w4: out {tuple(out.shape)} {out.dtype} on {out.device}: want [{M}, {N}] {x.dtype}")
-    a = abi.GemvW4Args(w=_ptr(w), scales=_ptr(scales), zeros=0 if zeros is None else _ptr(zeros), x=_ptr(x),
-                       y=_ptr(out), M=M, N=N, K=K, group=K // groups, x_ld=x_ld, y_ld=y_ld, f16=x.dtype is torch.float16)
-    need = ext.query("dsv41_gemv_w4_scratch_bytes", a)
-    if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.scratch, a.scratch_bytes = _ptr(scratch), need
-    ext.call("dsv41_gemv_w4", a, _stream())
+        out = torch.empty((M, N), dtype=dtype, device=x.device)
+    else:
+        y_ld, one = out.stride() if out.dim() == 2 else (0, 0)
+        if M < 2:
+            y_ld = N
+        if out.shape != (M, N) or out.dtype is not dtype or out.get_device() != dev or (N > 1 and one != 1) or y_ld < N:
+            raise RuntimeError(f"gemv_w4: out {tuple(out.shape)} {out.dtype} on {out.device} of strides {out.stride()}: "
+                               f"want [{M}, {N}] {dtype} on {x.device}, contiguous rows")
+        a.y_ld = y_ld
+    a.y = out.data_ptr()
+    if M > 16:  # fewer rows need no scratch
+        need = ext.query("dsv41_gemv_w4_scratch_bytes", a)
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+        a.scratch, a.scratch_bytes = scratch.data_ptr(), need
+    ext.call("dsv41_gemv_w4", a, stream)
     return out

@@ -21,12 +21,16 @@ from ...common import ext
 from . import abi
 
 DIMS = (64, 128, 256)
+_F32, _U32 = struct.Struct("<f"), struct.Struct("<I")
 
 
-def check_device(device: torch.device, name: str) -> None:
-    """Raise unless ``device`` is the current CUDA device, whose stream the launch goes to."""
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise RuntimeError(f"{name}: on {device}, which is not the current CUDA device")
+def current_stream(device: int, name: str) -> int:
+    """The current stream of CUDA device ``device``, which has to be the current device: the launch
+    goes there. (torch's own short way to both, a tenth of the public calls' time.)"""
+    if device < 0 or device != torch._C._cuda_getDevice():
+        where = "the host" if device < 0 else f"cuda:{device}"
+        raise RuntimeError(f"{name}: on {where}, which is not the current CUDA device")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 class PagedKV:
@@ -46,9 +50,11 @@ class PagedKV:
                                    f"{tuple(shape)} on {k.device}")
         self.k, self.v, self.k_codes, self.v_codes = k, v, k_codes, v_codes
         self.pages, self.kv_heads, self.page, self.dim, self.block = pages, heads, page, dim, page // per
+        self._dev = k.get_device()
+        self._scratch: dict = {}  # attention's scratch bytes by (heads, rows a sequence)
         cache = dict(kv_heads=heads, dim=dim, k_cache=k.data_ptr(), v_cache=v.data_ptr(), k_codes=k_codes.data_ptr(),
                      v_codes=v_codes.data_ptr(), pages=pages, page=page, block=self.block)
-        self._append_args, self._attend_args = abi.KvAppendArgs(**cache), abi.PagedAttnArgs(**cache)
+        self._append_args, self._attend_args = bytes(abi.KvAppendArgs(**cache)), bytes(abi.PagedAttnArgs(**cache))
 
     @classmethod
     def empty(cls, pages: int, page: int, kv_heads: int, dim: int, *, block: int = 16, device="cuda") -> "PagedKV":
@@ -61,46 +67,53 @@ class PagedKV:
                    torch.zeros(codes, **u8))
 
     # ------------------------------------------------------------ checks
-    def _rows(self, x: torch.Tensor, name: str, like: torch.Tensor, heads: int | None = None) -> int:
-        """Check rows [T, heads, dim] (a row's heads contiguous) and return their stride."""
-        shape, st = x.shape, x.stride()
-        if (len(shape) != 3 or shape[0] != like.shape[0] or shape[2] != self.dim or x.dtype != like.dtype
-                or (heads is not None and shape[1] != heads) or x.device != self.k.device):
-            raise RuntimeError(f"{name}: {tuple(shape)} {x.dtype} on {x.device}: want [{like.shape[0]}, "
-                               f"{heads or 'heads'}, {self.dim}] {like.dtype} on {self.k.device}")
-        ld = st[0] if shape[0] > 1 else max(st[0], shape[1] * self.dim)
-        ld = ld if shape[0] > 1 else -(-ld // 8) * 8
-        if st[2] != 1 or (st[1] != self.dim and shape[1] > 1) or ld % 8 or ld < shape[1] * self.dim \
-                or x.data_ptr() % 16:
-            raise RuntimeError(f"{name}: strides {st} at {x.data_ptr():#x}: a row's heads have to be contiguous, rows "
-                               "a multiple of 8 values apart and 16-byte aligned")
-        return ld
+    def _rows(self, x: torch.Tensor, name: str, rows: int, dtype: torch.dtype, heads: int) -> tuple[int, int]:
+        """Check rows [rows, heads, dim] (a row's heads contiguous): their address and their stride."""
+        dim, at = self.dim, x.data_ptr()
+        if x.shape != (rows, heads, dim) or x.dtype is not dtype or x.get_device() != self._dev:
+            raise RuntimeError(f"{name}: {tuple(x.shape)} {x.dtype} on {x.device}: want [{rows}, {heads}, {dim}] {dtype} "
+                               f"on {self.k.device}")
+        ld, head, one = x.stride()
+        if rows < 2:
+            ld = heads * dim
+        if one != 1 or (head != dim and heads > 1) or ld & 7 or ld < heads * dim or at & 15:
+            raise RuntimeError(f"{name}: strides {x.stride()} at {at:#x}: a row's heads have to be contiguous, rows a "
+                               "multiple of 8 values apart and 16-byte aligned")
+        return at, ld
 
-    def _step(self, a, x: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, cu_rows: torch.Tensor | None) -> None:
-        """Check the step's tensors and fill in what the two calls share."""
-        dev = self.k.device
-        check_device(dev, "PagedKV")
-        if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
-            raise RuntimeError(f"PagedKV: rows of {x.dtype}, want bfloat16 or float16")
-        i32 = torch.int32
-        seqs = lens.shape[0] if lens.dim() == 1 else -1
-        if seqs < 0 or lens.dtype != i32 or lens.device != dev or not lens.is_contiguous():
-            raise RuntimeError(f"lens: {tuple(lens.shape)} {lens.dtype} on {lens.device}: want [sequences] int32 on {dev}")
-        if table.dim() != 2 or table.shape[0] != seqs or table.shape[1] < 1 or table.dtype != i32 \
-                or table.device != dev or table.stride(1) != 1 or (seqs > 1 and table.stride(0) < table.shape[1]):
+    def _step(self, a, x: torch.Tensor, name: str, lens: torch.Tensor, table: torch.Tensor,
+              cu_rows: torch.Tensor | None) -> tuple[int, torch.dtype]:
+        """Check the step's tensors and fill in what the two calls share: (rows, their type)."""
+        dev, i32, dtype = self._dev, torch.int32, x.dtype
+        if x.dim() != 3:
+            raise RuntimeError(f"{name}: {tuple(x.shape)}: want [rows, heads, {self.dim}]")
+        if dtype is not torch.bfloat16 and dtype is not torch.float16:
+            raise RuntimeError(f"{name}: {dtype}, want bfloat16 or float16")
+        rows = x.shape[0]
+        if lens.dim() != 1 or lens.dtype is not i32 or lens.get_device() != dev or not lens.is_contiguous():
+            raise RuntimeError(f"lens: {tuple(lens.shape)} {lens.dtype} on {lens.device}: want [sequences] int32 on "
+                               f"{self.k.device}")
+        seqs = lens.shape[0]
+        if table.dim() != 2 or table.dtype is not i32 or table.get_device() != dev:
             raise RuntimeError(f"table: {tuple(table.shape)} {table.dtype} on {table.device}: want [{seqs}, pages] int32 "
-                               f"with contiguous rows on {dev}")
+                               f"on {self.k.device}")
+        n, width = table.shape
+        ld, one = table.stride()
+        if n != seqs or not width or (one != 1 and width > 1) or (ld < width and seqs > 1):
+            raise RuntimeError(f"table: {tuple(table.shape)} of strides {table.stride()}: want [{seqs}, pages] with "
+                               "contiguous rows")
         if cu_rows is None:
-            if seqs != x.shape[0]:
-                raise RuntimeError(f"{x.shape[0]} rows for {seqs} sequences without cu_rows: one row a sequence")
-        elif cu_rows.shape != (seqs + 1,) or cu_rows.dtype != i32 or cu_rows.device != dev \
+            if seqs != rows:
+                raise RuntimeError(f"{rows} rows for {seqs} sequences without cu_rows: one row a sequence")
+        elif cu_rows.shape != (seqs + 1,) or cu_rows.dtype is not i32 or cu_rows.get_device() != dev \
                 or not cu_rows.is_contiguous():
             raise RuntimeError(f"cu_rows: {tuple(cu_rows.shape)} {cu_rows.dtype} on {cu_rows.device}: want [{seqs + 1}] "
-                               f"int32 on {dev}")
-        a.T, a.seqs, a.f16 = x.shape[0], seqs, x.dtype is torch.float16
-        a.lens, a.table, a.width = lens.data_ptr(), table.data_ptr(), table.shape[1]
-        a.table_ld = max(table.stride(0), a.width)
-        a.cu_rows = 0 if cu_rows is None else cu_rows.data_ptr()
+                               f"int32 on {self.k.device}")
+        else:
+            a.cu_rows = cu_rows.data_ptr()
+        a.T, a.seqs, a.f16, a.lens, a.table = rows, seqs, dtype is torch.float16, lens.data_ptr(), table.data_ptr()
+        a.width, a.table_ld = width, ld if seqs > 1 else width
+        return rows, dtype
 
     # ------------------------------------------------------------ operators
     def append(self, k: torch.Tensor, v: torch.Tensor, *, lens: torch.Tensor, table: torch.Tensor,
@@ -114,31 +127,33 @@ class PagedKV:
         pairs (2j, 2j + 1) or, ``neox``, (j, j + rope / 2). Returns the rotated queries (``q_out``,
         which may be ``q``, or a new tensor), or None without ``q``. A sequence's pages must not be
         another's: two sequences that append to one block race."""
+        stream = current_stream(self._dev, "PagedKV.append")
         a = abi.KvAppendArgs.from_buffer_copy(self._append_args)
-        if k.dim() != 3:
-            raise RuntimeError(f"k: {tuple(k.shape)}: want [rows, {self.kv_heads}, {self.dim}]")
-        self._step(a, k, lens, table, cu_rows)
-        a.k, a.k_ld = k.data_ptr(), self._rows(k, "k", k, self.kv_heads)
-        a.v, a.v_ld = v.data_ptr(), self._rows(v, "v", k, self.kv_heads)
-        a.heads = self.kv_heads
+        rows, dtype = self._step(a, k, "k", lens, table, cu_rows)
+        heads = self.kv_heads
+        a.k, a.k_ld = self._rows(k, "k", rows, dtype, heads)
+        a.v, a.v_ld = self._rows(v, "v", rows, dtype, heads)
         if cos_sin is not None:
-            if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.device != self.k.device \
+            if cos_sin.dim() != 2 or cos_sin.dtype is not torch.float32 or cos_sin.get_device() != self._dev \
                     or not cos_sin.is_contiguous() or not cos_sin.shape[0] or cos_sin.shape[1] % 16 \
-                    or not 16 <= cos_sin.shape[1] <= self.dim or cos_sin.data_ptr() % 16:
+                    or not 16 <= cos_sin.shape[1] <= self.dim or cos_sin.data_ptr() & 15:
                 raise RuntimeError(f"cos_sin: {tuple(cos_sin.shape)} {cos_sin.dtype} on {cos_sin.device}: want "
                                    f"[positions, rope] fp32, rope a multiple of 16 up to {self.dim}")
-            a.cos_sin, a.rope_rows, a.rope, a.neox = cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1], bool(neox)
+            a.cos_sin = cos_sin.data_ptr()
+            a.rope_rows, a.rope = cos_sin.shape
+            a.neox = bool(neox)
         if q is not None:
-            a.q, a.q_ld = q.data_ptr(), self._rows(q, "q", k)
-            a.heads = q.shape[1]
-            if not a.heads or a.heads % self.kv_heads:
-                raise RuntimeError(f"q: {a.heads} heads over {self.kv_heads} key heads")
+            if q.dim() != 3 or not q.shape[1] or q.shape[1] % heads:
+                raise RuntimeError(f"q: {tuple(q.shape)}: want [{rows}, heads, {self.dim}], heads a multiple of {heads}")
+            heads = q.shape[1]
+            a.q, a.q_ld = self._rows(q, "q", rows, dtype, heads)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            a.q_out, a.q_out_ld = q_out.data_ptr(), self._rows(q_out, "q_out", k, a.heads)
+                q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+            a.q_out, a.q_out_ld = self._rows(q_out, "q_out", rows, dtype, heads)
         elif q_out is not None:
             raise RuntimeError("q_out without q")
-        ext.call("dsv41_kv_append", a, torch.cuda.current_stream().cuda_stream)
+        a.heads = heads
+        ext.call("dsv41_kv_append", a, stream)
         return q_out
 
     def attend(self, q: torch.Tensor, *, lens: torch.Tensor, table: torch.Tensor, scale: float,
@@ -150,28 +165,32 @@ class PagedKV:
         softmax, with ``sink`` [heads] fp32 as one more score without a value. A row that sees
         nothing gives zeros. Returns ``out`` (or a new tensor) [T, heads, dim]; rows behind the last
         sequence are left as they were."""
+        stream = current_stream(self._dev, "PagedKV.attend")
         a = abi.PagedAttnArgs.from_buffer_copy(self._attend_args)
-        if q.dim() != 3:
-            raise RuntimeError(f"q: {tuple(q.shape)}: want [rows, heads, {self.dim}]")
-        self._step(a, q, lens, table, cu_rows)
-        a.q, a.q_ld = q.data_ptr(), self._rows(q, "q", q)
-        a.heads = heads = q.shape[1]
+        rows, dtype = self._step(a, q, "q", lens, table, cu_rows)
+        heads = q.shape[1]
         if not heads or heads % self.kv_heads:
             raise RuntimeError(f"q: {heads} heads over {self.kv_heads} key heads")
+        a.heads = heads
+        a.q, a.q_ld = self._rows(q, "q", rows, dtype, heads)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        a.out, a.out_ld = out.data_ptr(), self._rows(out, "out", q, heads)
+            out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        a.out, a.out_ld = self._rows(out, "out", rows, dtype, heads)
         if not 0 <= window < 1 << 31:
             raise RuntimeError(f"window {window}")
         a.window = window
         if sink is not None:
-            if sink.shape != (heads,) or sink.dtype != torch.float32 or sink.device != q.device \
+            if sink.shape != (heads,) or sink.dtype is not torch.float32 or sink.get_device() != self._dev \
                     or not sink.is_contiguous():
                 raise RuntimeError(f"sink: {tuple(sink.shape)} {sink.dtype} on {sink.device}: want [{heads}] fp32")
             a.sink = sink.data_ptr()
-        a.scale_f32 = struct.unpack("<I", struct.pack("<f", scale))[0]
-        need = ext.query("dsv41_paged_attn_scratch_bytes", a)
+        a.scale_f32 = _U32.unpack(_F32.pack(scale))[0]
+        # the scratch depends on the heads and on the rows a sequence has on average
+        key = heads, -(-rows // a.seqs) if a.seqs else 0
+        need = self._scratch.get(key)
+        if need is None:
+            need = self._scratch[key] = ext.query("dsv41_paged_attn_scratch_bytes", a)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
         a.scratch, a.scratch_bytes = scratch.data_ptr(), need
-        ext.call("dsv41_paged_attn", a, torch.cuda.current_stream().cuda_stream)
+        ext.call("dsv41_paged_attn", a, stream)
         return out
