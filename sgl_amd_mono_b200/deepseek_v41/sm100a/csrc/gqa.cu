@@ -61,7 +61,7 @@ bool attn_ok(const Dsv41PagedAttnArgs* a) {
 // accumulators that fit: 32 columns of 64 or 128 dims, 16 of 256.
 int attn_tiles(const Dsv41PagedAttnArgs* a) {
   const int64_t cols = a->heads / a->kv_heads * std::max<int64_t>(1, cdiv64(a->T, std::max<int64_t>(1, a->seqs)));
-  return cols <= 8 ? 1 : cols <= 16 || a->dim == 256 ? 2 : 4;
+  return cols <= 8 ? 1 : cols <= 16 || a->dim == 256 ? 2 : cols <= 24 ? 3 : 4;
 }
 
 template <int V>
@@ -75,6 +75,7 @@ int64_t attn_go(const Dsv41PagedAttnArgs* a, F f) {
     switch (attn_tiles(a)) {
       case 1: return by_type(d, Int<1>());
       case 2: return by_type(d, Int<2>());
+      case 3: return by_type(d, Int<d == 256 ? 2 : 3>());
       default: return by_type(d, Int<d == 256 ? 2 : 4>());
     }
   };
@@ -87,7 +88,7 @@ int64_t attn_ctas() {
 }
 template <int D, int NT>
 int64_t attn_scratch() {
-  return 2 * attn_ctas<D, NT>() * 8 * NT * (D * sizeof(float) + sizeof(float4));
+  return attn_ctas<D, NT>() * (2 * 8 * NT * (D * sizeof(float) + sizeof(float4)) + sizeof(PaSplit));
 }
 
 template <int F16, int D, int NT>
@@ -100,10 +101,11 @@ int attn_run(const Dsv41PagedAttnArgs* a, void* stream) {
   float* part = ptr<float>(a->scratch);
   const PagedAttnArgs p = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->window, scale * 1.44269504f,
                            ptr<const void>(a->q), ptr<void>(a->out), a->q_ld, a->out_ld, ptr<const float>(a->sink),
-                           part, reinterpret_cast<float4*>(part + slots * D)};
-  const int rc = launch(paged_attn_kernel<F16, D, NT>, dim3((unsigned)ctas), dim3(32 * kPaWarps),
+                           part, reinterpret_cast<float4*>(part + slots * D),
+                           reinterpret_cast<PaSplit*>(part + slots * (D + 4))};
+  const int rc = launch(paged_attn_kernel<F16, D, NT>, dim3((unsigned)ctas), dim3(32 * PaShape<D, NT>::kWarps),
                         PaShape<D, NT>::kBytes, stream, p);
-  return rc ? rc : launch(paged_join_kernel<F16, D, NT>, dim3((unsigned)ctas), dim3(32 * kPaWarps), 0, stream, p);
+  return rc ? rc : launch(paged_join_kernel<F16, D, NT>, dim3((unsigned)ctas, 8 * NT), dim3(kPaJoinThreads), 0, stream, p);
 }
 
 }  // namespace

@@ -32,8 +32,6 @@
 
 namespace dsv41 {
 
-constexpr int kPaWarps = 8;
-
 struct PagedAttnArgs {
   StepRows rows;
   KvCache cache;
@@ -45,6 +43,13 @@ struct PagedAttnArgs {
   const float* sink;  // [heads] or null
   float* part;        // [2 CTAs][8 NT][dim] unnormalised pieces
   float4* part_rl;    // [2 CTAs][8 NT] their references r and c and their sum
+  struct PaSplit* split;  // [CTAs]
+};
+
+// The item that begins in a share and goes on in the next ones, if one does: its pieces (0: none), what
+// its columns are, and the slot of its first piece (the others lie in the slots 2 (share + i)).
+struct PaSplit {
+  int pieces, slot, row0, h0, col0, cols, pad[2];
 };
 
 // One sequence's work: its rows, its tiles [tile0, tile0 + tiles) and what that makes in units.
@@ -53,7 +58,7 @@ struct SeqWork {
   long long units;
 };
 
-template <int NT>
+template <int NT, int W>
 __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
   SeqWork w;
   w.row0 = a.rows.cu_rows ? a.rows.cu_rows[s] : s;
@@ -67,27 +72,27 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
   const int lo = a.window ? max(0, w.end - w.n + 1 - a.window) : 0;
   w.tile0 = lo / 16;
   w.tiles = max(0, (hi + 15) / 16 - w.tile0);
-  w.steps = max(1, (w.tiles + kPaWarps - 1) / kPaWarps);
+  w.steps = max(1, (w.tiles + W - 1) / W);
   w.units = (long long)w.cts * kvh * w.steps;
   return w;
 }
 
 // The whole work and this share of it: seq and unit where share `c` of `shares` begins, found by all
-// threads of a 32 kPaWarps CTA. per = units a share.
+// threads of a CTA of W warps. per = units a share.
 struct Share {
   long long first, last, per;  // units [first, last)
   int seq;                     // the sequence of unit `first`
   long long seq0;              // its first unit
 };
 
-template <int NT>
+template <int NT, int W>
 __device__ __forceinline__ Share find_share(const PagedAttnArgs& a, int c, int shares, long long* sm) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kThreads = 32 * kPaWarps;
+  constexpr int kThreads = 32 * W;
   const int seqs = a.rows.seqs;
   // the units before each thread's sequence, a chunk of kThreads sequences at a time
   auto scan = [&](int base, long long& before, long long& own) {
-    own = base + tid < seqs ? seq_work<NT>(a, base + tid).units : 0;
+    own = base + tid < seqs ? seq_work<NT, W>(a, base + tid).units : 0;
     long long x = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -100,7 +105,7 @@ __device__ __forceinline__ Share find_share(const PagedAttnArgs& a, int c, int s
     before = x - own;
     long long all = 0;
 #pragma unroll
-    for (int i = 0; i < kPaWarps; ++i) {
+    for (int i = 0; i < W; ++i) {
       if (i < warp) before += sm[i];
       all += sm[i];
     }
@@ -125,13 +130,13 @@ __device__ __forceinline__ Share find_share(const PagedAttnArgs& a, int c, int s
       sum += all;
     }
     if (own && before <= r.first && r.first < before + own) {
-      sm[kPaWarps] = base + tid;
-      sm[kPaWarps + 1] = before;
+      sm[W] = base + tid;
+      sm[W + 1] = before;
     }
   }
   __syncthreads();
-  r.seq = (int)sm[kPaWarps];
-  r.seq0 = sm[kPaWarps + 1];
+  r.seq = (int)sm[W];
+  r.seq0 = sm[W + 1];
   return r;
 }
 
@@ -159,22 +164,37 @@ __device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t& lo, uint32_t& h
       : "=r"(lo), "=r"(hi)
       : "r"(w));
 }
-// Whether a byte of w is an e4m3 NaN.
-__device__ __forceinline__ bool has_nan(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0; }
+// m16n8k16 of f16 and a shared-memory load that the compiler may schedule freely.
+__device__ __forceinline__ void pa_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <class V>
+__device__ __forceinline__ V pa_lds(const uint8_t* p) {
+  return *reinterpret_cast<const V*>(p);
+}
+// The bytes of w that are e4m3 NaN, as a mask.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
 template <int D, int NT>
 struct PaShape {
-  static constexpr int kRegs = NT * D;              // O registers a thread: kRegs / 4
-  static constexpr int kCtas = kRegs <= 128 ? 2 : 1;  // an SM
-  static constexpr int kTile = 32 * D;              // bytes of a staged tile, K and V
-  static constexpr int kStagesFit = (kCtas == 2 ? 96 : 192) * 1024 / (kPaWarps * kTile);
+  // What a thread holds decides how many warps an SM runs: two CTAs of 8 while O takes up to 32 registers
+  // (and the fragments of Q as many), one of 12 up to 96, else one of 8 (8 sequences of 4 rows and 4 heads
+  // a kv head at 32768 tokens, O of 64: 121 us with 12 warps, 125 with two CTAs of 8, 140 with 8).
+  static constexpr int kO = NT * D / 4;               // O registers a thread
+  static constexpr int kCtas = kO <= 32 ? 2 : 1;      // an SM
+  static constexpr int kWarps = kO <= 32 || kO > 96 ? 8 : 12;
+  static constexpr int kTile = 32 * D;                // bytes of a staged tile, K and V
+  static constexpr int kStagesFit = 192 / kCtas * 1024 / (kWarps * kTile);
   static constexpr int kStages = kStagesFit > 6 ? 6 : kStagesFit;
-  static constexpr bool kQSmem = kRegs > 256;       // Q fragments re-read from shared memory
-  static constexpr int kRing = kPaWarps * kStages * kTile;
+  static constexpr bool kQSmem = kO > 32;             // Q fragments re-read from shared memory
+  static constexpr int kRing = kWarps * kStages * kTile;
   static constexpr int kQBytes = kQSmem ? 8 * NT * D * 2 : 0;
-  static constexpr int kRl = kPaWarps * 8 * NT * 16;  // the warps' references and sums
-  static constexpr int kBytes = kRing + kQBytes + kRl + (kPaWarps + 2) * 8;
-  static_assert(kPaWarps / 2 * 8 * NT * D * 4 <= kRing, "the merge reuses the ring");
+  static constexpr int kRl = kWarps * 8 * NT * 16;    // the warps' references and sums
+  static constexpr int kBytes = kRing + kQBytes + kRl + (kWarps + 2) * 8;
+  static_assert(kWarps / 2 * 8 * NT * D * 4 <= kRing, "the merge reuses the ring");
 };
 
 // What turns sum_i w_i V_i into the output: 2^(r - 7 - c) over the sum (0 where nothing was seen).
@@ -190,47 +210,55 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 }
 
 template <bool F16, int D, int NT>
-__global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_attn_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::kCtas) paged_attn_kernel(const PagedAttnArgs a) {
   using P = PaShape<D, NT>;
   using T = typename Act<F16>::T;
-  constexpr int W = kPaWarps, S = P::kStages, KS = D / 16;
+  constexpr int W = P::kWarps, S = P::kStages, KS = D / 16;
   extern __shared__ __align__(128) uint8_t pa_smem[];
   uint2* q_sm = reinterpret_cast<uint2*>(pa_smem + P::kRing);
   float4* rl_sm = reinterpret_cast<float4*>(pa_smem + P::kRing + P::kQBytes);
   long long* plan_sm = reinterpret_cast<long long*>(pa_smem + P::kRing + P::kQBytes + P::kRl);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem_u32(pa_smem) + warp * S * P::kTile;
+  uint8_t* ring_p = pa_smem + warp * S * P::kTile;
+  const uint32_t ring = smem_u32(ring_p);
   const int kvh = a.cache.kv_heads, group = a.heads / kvh, page = a.cache.page, block = a.cache.block;
   const int kap = pa_kappa(g);
 
   pdl_wait();
   pdl_launch();
-  const Share sh = find_share<NT>(a, blockIdx.x, gridDim.x, plan_sm);
+  if (tid == 0) a.split[blockIdx.x].pieces = 0;
+  const Share sh = find_share<NT, W>(a, blockIdx.x, gridDim.x, plan_sm);
   if (sh.seq < 0) return;
-  int seq = sh.seq;
-  SeqWork w = seq_work<NT>(a, seq);
-  long long seq0 = sh.seq0;
-  for (long long u = sh.first; u < sh.last;) {
-    while (u >= seq0 + w.units) {
-      seq0 += w.units;
-      w = seq_work<NT>(a, ++seq);
+  // Where the share stands lies in shared memory between pieces, not in registers: the sequence, the
+  // unit in it, the units left.
+  if (tid == 0) plan_sm[0] = sh.seq, plan_sm[1] = sh.first - sh.seq0, plan_sm[2] = sh.last - sh.first, plan_sm[3] = sh.per;
+  for (bool first_piece = true;; first_piece = false) {
+    __syncthreads();
+    int seq = (int)plan_sm[0];
+    long long at = plan_sm[1];
+    const long long left = plan_sm[2];
+    if (left <= 0) break;
+    SeqWork w = seq_work<NT, W>(a, seq);
+    while (at >= w.units) {
+      at -= w.units;
+      w = seq_work<NT, W>(a, ++seq);
     }
     // this piece: kv head hk, column tile ct, steps [step0, step1)
-    const int item = (int)((u - seq0) / w.steps), step0 = (int)((u - seq0) % w.steps);
-    const int step1 = (int)min((long long)w.steps, step0 + sh.last - u);
+    const int item = (int)(at / w.steps), step0 = (int)(at % w.steps);
+    const int step1 = (int)min((long long)w.steps, step0 + left);
     const int ct = item % w.cts, hk = item / w.cts;
     const int col0 = ct * 8 * NT;
     // what its first and last row see
     const int j0 = col0 / group, j1 = (min(col0 + 8 * NT, w.cols) - 1) / group;
     const int cap = a.rows.width * page;
-    auto vis = [&](int j) { return w.end - w.n + j + 1; };
+    const int vis0 = w.end - w.n + 1;
+    auto vis = [&](int j) { return vis0 + j; };
     auto low = [&](int j) { return a.window ? max(0, vis(j) - a.window) : 0; };
     const int any_lo = low(j0), any_hi = min(vis(j1), cap), all_lo = low(j1), all_hi = min(vis(j0), cap);
 
     // Q: column n's dims 64 c + 16 t + 4 q + {0 .. 3} are step 4 c + q's fragment of lane (n, t)
     uint32_t qf[P::kQSmem ? 1 : NT][P::kQSmem ? 1 : KS][2];
     float qmul[NT][2];
-    if (P::kQSmem) __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int col = col0 + 8 * n + g;
@@ -312,9 +340,10 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
     // one before (prev): page, or -1 where the piece sees none of the tile's tokens
     int cur_pg = -1, prev_pg = -1;
     uint32_t cur_sc = 0, prev_sc = 0;
+    const int tile_first = w.tile0 + first;
     auto load_batch = [&](int b) {
       prev_pg = cur_pg, prev_sc = cur_sc;
-      const int j = 32 * b + lane, p0 = (w.tile0 + first + W * j) * 16;
+      const int j = 32 * b + lane, p0 = (tile_first + W * j) * 16;
       cur_pg = -1;
       if (j < count && p0 < any_hi && p0 + 16 > any_lo) {
         cur_pg = token_page(a.rows, a.cache, seq, p0);
@@ -329,7 +358,7 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
         if (j % 32 == 0) load_batch(j / 32);
         const int pg = __shfl_sync(0xffffffffu, cur_pg, j & 31);
         if (pg >= 0) {
-          const int64_t at = (((int64_t)pg * kvh + hk) * page + (w.tile0 + first + W * j) * 16 % page) * D;
+          const int64_t at = (((int64_t)pg * kvh + hk) * page + (tile_first + W * j) * 16 % page) * D;
           const uint32_t dst = ring + j % S * P::kTile;
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
@@ -354,17 +383,22 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
       const int pg = __shfl_sync(0xffffffffu, is_cur ? cur_pg : prev_pg, j & 31);
       const uint32_t sc = __shfl_sync(0xffffffffu, is_cur ? cur_sc : prev_sc, j & 31);
       if (pg < 0) continue;
-      const uint32_t kt = ring + j % S * P::kTile, vt = kt + 16 * D;
-      const int p0 = (w.tile0 + first + W * j) * 16;
+      const uint8_t *kt = ring_p + j % S * P::kTile, *vt = kt + 16 * D;
+      const int p0 = (tile_first + W * j) * 16;
       const bool edge = p0 < all_lo || p0 + 16 > all_hi;
 
       // S^T = K Q^T
-      float s[NT][4];
+      // (QC chains a column tile: one tensor-core instruction waits for the one before it in its chain)
+      constexpr int QC = NT <= 2 ? 2 : 1;
+      float sq[QC][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int x = 0; x < QC; ++x)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sq[x][n][0] = sq[x][n][1] = sq[x][n][2] = sq[x][n][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        const uint4 x = lds16(kt + pa_chunk<D>(kap, 4 * c + t)), y = lds16(kt + pa_chunk<D>(kap + 8, 4 * c + t));
+        const uint4 x = pa_lds<uint4>(kt + pa_chunk<D>(kap, 4 * c + t));
+        const uint4 y = pa_lds<uint4>(kt + pa_chunk<D>(kap + 8, 4 * c + t));
         const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -377,10 +411,18 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
             if (P::kQSmem) b = q_sm[(n * KS + 4 * c + i) * 32 + lane];
             else b = make_uint2(qf[P::kQSmem ? 0 : n][P::kQSmem ? 0 : 4 * c + i][0],
                                 qf[P::kQSmem ? 0 : n][P::kQSmem ? 0 : 4 * c + i][1]);
-            mma_f16(s[n], a0, a1, a2, a3, b.x, b.y);
+            pa_mma(sq[i % QC][n], a0, a1, a2, a3, b.x, b.y);
           }
         }
       }
+
+      float(&s)[NT][4] = sq[0];
+#pragma unroll
+      for (int x = 1; x < QC; ++x)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] += sq[x][n][e];
 
       // s: scores, base 2; elements (token kappa, column 2t), (kappa, 2t + 1), (kappa + 8, ..)
       const float ks = pow2c(sc & 255), ev = (float)((int)(sc >> 8) - 127);
@@ -390,12 +432,15 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] *= qmul[n][e & 1] * ks;
       if (edge) {
+        int c0 = col0 + 2 * t;
+        asm volatile("" : "+r"(c0));  // nothing of this branch is to be kept in registers from tile to tile
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = (col0 + 8 * n + 2 * t + (e & 1)) / group, p = p0 + kap + (e >> 1) * 8;
-            if (p >= min(vis(j), cap) || p < low(j)) s[n][e] = -INFINITY;
+          for (int e = 0; e < 2; ++e) {
+            const int j = (c0 + 8 * n + e) / group, hi = min(vis(j), cap), lo = low(j), p = p0 + kap;
+            if (p >= hi || p < lo) s[n][e] = -INFINITY;
+            if (p + 8 >= hi || p + 8 < lo) s[n][e + 2] = -INFINITY;
           }
       }
 #pragma unroll
@@ -437,74 +482,67 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
       for (int r = 0; r < 4; ++r) {
         const int row = ((r & 1) ? 7 - t : t) + (r >> 1) * 8;
         if (D == 64) {
-          const uint2 x = lds8(vt + pa_chunk<D>(row, g >> 1) + (g & 1) * 8);
+          const uint2 x = pa_lds<uint2>(vt + pa_chunk<D>(row, g >> 1) + (g & 1) * 8);
           v[r][0] = x.x, v[r][1] = x.y;
         } else {
 #pragma unroll
           for (int c = 0; c < D / 128; ++c) {
-            const uint4 x = lds16(vt + pa_chunk<D>(row, 8 * c + ((g >> 1) | (g & 1) << 2)));
+            const uint4 x = pa_lds<uint4>(vt + pa_chunk<D>(row, 8 * c + ((g >> 1) | (g & 1) << 2)));
             v[r][4 * c] = x.x, v[r][4 * c + 1] = x.y, v[r][4 * c + 2] = x.z, v[r][4 * c + 3] = x.w;
           }
         }
       }
-      auto pv = [&](const uint32_t (&vv)[4][D / 32], float (&acc)[NT][KS][4]) {
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t a0, a1, a2, a3;
-            const uint32_t sel = h ? 0x7362 : 0x5140;  // (x_2h, y_2h, x_2h+1, y_2h+1)
-            e4m3x4_f16(__byte_perm(vv[0][i], vv[1][i], sel), a0, a1);
-            e4m3x4_f16(__byte_perm(vv[2][i], vv[3][i], sel), a2, a3);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(acc[n][2 * i + h], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-          }
-      };
-      bool row_by_row = false;
+      bool nan = false;
       if (edge) {
-        // tokens that no row of the piece sees hold anything; NaN in one that only some rows see
-        // must not reach the others as 0 NaN
-        bool nan = false;
+        // tokens that no row of the piece sees hold anything; NaN in one that only some rows see must not
+        // reach the others as 0 NaN, so NaN bytes go in as zeros here and come back below
+        int p1 = p0;
+        asm volatile("" : "+r"(p1));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int p = p0 + ((r & 1) ? 7 - t : t) + (r >> 1) * 8;
+          const int p = p1 + ((r & 1) ? 7 - t : t) + (r >> 1) * 8;
           const bool seen = p >= any_lo && p < any_hi;
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
-            v[r][i] = seen ? v[r][i] : 0u;
-            nan |= has_nan(v[r][i]);
+            const uint32_t m = nan_bytes(v[r][i]);
+            nan |= seen && m;
+            v[r][i] = seen ? v[r][i] & ~m : 0u;
           }
         }
-        row_by_row = __any_sync(0xffffffffu, nan);
       }
-      if (!row_by_row) {
-        pv(v, o);
-      } else {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a0, a1, a2, a3;
+          const uint32_t sel = h ? 0x7362 : 0x5140;  // (x_2h, y_2h, x_2h+1, y_2h+1)
+          e4m3x4_f16(__byte_perm(v[0][i], v[1][i], sel), a0, a1);
+          e4m3x4_f16(__byte_perm(v[2][i], v[3][i], sel), a2, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) pa_mma(o[n][2 * i + h], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        }
+      if (edge && __any_sync(0xffffffffu, nan)) {
+        // this lane's dims of each token again: what holds NaN makes NaN of the columns that see it
 #pragma unroll 1
-        for (int j = j0; j <= j1; ++j) {
-          uint32_t vj[4][D / 32];
+        for (int r = 0; r < 16; ++r) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int p = p0 + ((r & 1) ? 7 - t : t) + (r >> 1) * 8;
-            const bool seen = p >= low(j) && p < min(vis(j), cap);
+          for (int i = 0; i < D / 32; ++i) {
+            const uint8_t* x = D == 64 ? vt + pa_chunk<D>(r, g >> 1) + (g & 1) * 8 + 4 * i
+                                       : vt + pa_chunk<D>(r, 8 * (i / 4) + ((g >> 1) | (g & 1) << 2)) + 4 * (i & 3);
+            const uint32_t m = nan_bytes(pa_lds<uint32_t>(x));
+            if (!m) continue;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) vj[r][i] = seen ? v[r][i] : 0u;
-          }
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int c = col0 + 8 * n + 2 * t;
-            const bool mine[2] = {c / group == j, (c + 1) / group == j};
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-              uint32_t a0, a1, a2, a3;
-              const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
-              e4m3x4_f16(__byte_perm(vj[0][i / 2], vj[1][i / 2], sel), a0, a1);
-              e4m3x4_f16(__byte_perm(vj[2][i / 2], vj[3][i / 2], sel), a2, a3);
-              float x[4] = {};
-              mma_f16(x, a0, a1, a2, a3, pb[n][0], pb[n][1]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[n][i][e] += mine[e & 1] ? x[e] : 0.f;
-            }
+              for (int e = 0; e < 2; ++e) {
+                const int j = (col0 + 8 * n + 2 * t + e) / group;
+                if (p0 + r >= min(vis(j), cap) || p0 + r < low(j)) continue;
+                const float bad = __uint_as_float(0x7fffffffu);
+                if (m & 0xffu) o[n][2 * i][e] = bad;
+                if (m & 0xff00u) o[n][2 * i][e + 2] = bad;
+                if (m & 0xff0000u) o[n][2 * i + 1][e] = bad;
+                if (m & 0xff000000u) o[n][2 * i + 1][e + 2] = bad;
+              }
           }
         }
       }
@@ -551,8 +589,9 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
       }
     float4* mb = reinterpret_cast<float4*>(pa_smem);
 #pragma unroll
-    for (int half = W / 2; half >= 1; half >>= 1) {
-      if (warp >= half && warp < 2 * half)
+    for (int n_w = W; n_w > 1; n_w = (n_w + 1) / 2) {
+      const int half = (n_w + 1) / 2;
+      if (warp >= half && warp < n_w)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -560,7 +599,7 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
             mb[(((warp - half) * NT + n) * KS + i) * 32 + lane] =
                 make_float4(o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]);
       __syncthreads();
-      if (warp < half)
+      if (warp < n_w - half)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -571,7 +610,11 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
       __syncthreads();
     }
     const bool whole = step0 == 0 && step1 == w.steps;
-    const int slot = 2 * blockIdx.x + (u == sh.first ? 0 : 1);
+    const int slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
+    if (tid == 0 && step0 == 0 && !whole) {
+      const long long per = plan_sm[3];
+      a.split[blockIdx.x] = {1 + (int)((w.steps - step1 + per - 1) / per), slot, w.row0, hk * group, col0, w.cols};
+    }
     if (warp == 0)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -604,58 +647,66 @@ __global__ void __launch_bounds__(32 * kPaWarps, PaShape<D, NT>::kCtas) paged_at
             }
           }
         }
-    u += step1 - step0;
+    if (tid == 0) plan_sm[0] = seq, plan_sm[1] = at + (step1 - step0), plan_sm[2] = left - (step1 - step0);
   }
 }
 
-// Join the pieces of the item that begins in share blockIdx.x and goes on past its end (at most one),
-// in the order of the shares. Thread = (column, 4 dims) in turn.
+constexpr int kPaJoinThreads = 128;
+
+// Join the pieces of the item that begins in share blockIdx.x and goes on past its end (at most one): one
+// CTA a column. The pieces are summed D / 4 threads a piece, several at a time, and those sums in order.
 template <bool F16, int D, int NT>
-__global__ void __launch_bounds__(32 * kPaWarps) paged_join_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const PagedAttnArgs a) {
   using T = typename Act<F16>::T;
-  __shared__ long long plan_sm[kPaWarps + 2];
+  constexpr int LG = D / 4, PG = kPaJoinThreads / LG;  // threads a piece, pieces at a time
+  __shared__ float red[3][kPaJoinThreads / 32];
+  __shared__ float4 sums[PG][LG];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.y;
   pdl_wait();
-  const int c = blockIdx.x, kvh = a.cache.kv_heads, group = a.heads / kvh;
-  Share sh = find_share<NT>(a, c, gridDim.x, plan_sm);
-  if (sh.seq < 0) return;
-  int seq = sh.seq;
-  SeqWork w = seq_work<NT>(a, seq);
-  long long seq0 = sh.seq0;
-  while (sh.last > seq0 + w.units) {
-    seq0 += w.units;
-    w = seq_work<NT>(a, ++seq);
+  const PaSplit sp = a.split[blockIdx.x];
+  if (!sp.pieces || sp.col0 + c >= sp.cols) return;
+  auto at = [&](int i) { return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : sp.slot) * 8 * NT + c; };
+  float m = -FLT_MAX, top = -FLT_MAX, sum = 0.f;
+  for (int i = tid; i < sp.pieces; i += kPaJoinThreads) {
+    const float4 rl = a.part_rl[at(i)];
+    m = fmaxf(m, rl.x);
+    top = fmaxf(top, rl.y);
   }
-  const int item = (int)((sh.last - 1 - seq0) / w.steps);
-  const long long u0 = seq0 + (long long)item * w.steps, u1 = u0 + w.steps;
-  if (u0 < sh.first || u1 <= sh.last) return;
-  const int pieces = (int)((u1 - 1) / sh.per) - c + 1;
-  const int ct = item % w.cts, hk = item / w.cts, col0 = ct * 8 * NT;
-  auto slot = [&](int i) { return (int64_t)2 * (c + i) + (i == 0 && u0 != sh.first ? 1 : 0); };
-  for (int x = threadIdx.x; x < 8 * NT * (D / 4); x += blockDim.x) {
-    const int cc = x / (D / 4), d = x % (D / 4) * 4, col = col0 + cc;
-    if (col >= w.cols) break;
-    float m = -FLT_MAX, top = -FLT_MAX, sum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const float4 rl = a.part_rl[slot(i) * 8 * NT + cc];
-      m = fmaxf(m, rl.x);
-      top = fmaxf(top, rl.y);
-    }
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const float4 rl = a.part_rl[slot(i) * 8 * NT + cc];
-      const float4 y = *reinterpret_cast<const float4*>(a.part + (slot(i) * 8 * NT + cc) * D + d);
-      const float f = ex2(rl.x - m);
-      sum = fmaf(rl.z, ex2(rl.y - top), sum);
-      o.x = fmaf(y.x, f, o.x), o.y = fmaf(y.y, f, o.y), o.z = fmaf(y.z, f, o.z), o.w = fmaf(y.w, f, o.w);
-    }
-    const int h = hk * group + col % group;
-    if (a.sink) sum += ex2(a.sink[h] * 1.44269504f - top);
-    const float f = pa_factor(m, top, sum);
-    T* y = reinterpret_cast<T*>(a.out) + (w.row0 + col / group) * a.out_ld + h * D + d;
-    *reinterpret_cast<uint2*>(y) = make_uint2(Act<F16>::pack(o.x * f, o.y * f), Act<F16>::pack(o.z * f, o.w * f));
+  m = warp_max(m), top = warp_max(top);
+  if (lane == 0) red[0][warp] = m, red[1][warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPaJoinThreads / 32; ++w) m = fmaxf(m, red[0][w]), top = fmaxf(top, red[1][w]);
+  for (int i = tid; i < sp.pieces; i += kPaJoinThreads) {
+    const float4 rl = a.part_rl[at(i)];
+    sum = fmaf(rl.z, ex2(rl.y - top), sum);
   }
+  sum = warp_sum(sum);
+  if (lane == 0) red[2][warp] = sum;
+  const int d = tid % LG, pg = tid / LG;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = pg; i < sp.pieces; i += PG) {
+    const float f = ex2(a.part_rl[at(i)].x - m);
+    const float4 y = *reinterpret_cast<const float4*>(a.part + at(i) * D + 4 * d);
+    o.x = fmaf(y.x, f, o.x), o.y = fmaf(y.y, f, o.y), o.z = fmaf(y.z, f, o.z), o.w = fmaf(y.w, f, o.w);
+  }
+  sums[pg][d] = o;
+  __syncthreads();
+  if (pg) return;
+#pragma unroll
+  for (int i = 1; i < PG; ++i) {
+    const float4 y = sums[i][d];
+    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+  }
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kPaJoinThreads / 32; ++w) sum += red[2][w];
+  const int col = sp.col0 + c, group = a.heads / a.cache.kv_heads, h = sp.h0 + col % group;
+  if (a.sink) sum += ex2(a.sink[h] * 1.44269504f - top);
+  const float f = pa_factor(m, top, sum);
+  T* y = reinterpret_cast<T*>(a.out) + (int64_t)(sp.row0 + col / group) * a.out_ld + h * D + 4 * d;
+  *reinterpret_cast<uint2*>(y) = make_uint2(Act<F16>::pack(o.x * f, o.y * f), Act<F16>::pack(o.z * f, o.w * f));
 }
 
 }  // namespace dsv41

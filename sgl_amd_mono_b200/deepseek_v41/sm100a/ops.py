@@ -67,7 +67,7 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch
                                f"uint8 on {x.device}")
         a.zeros = zeros.data_ptr()
     if out is None:
-        out = torch.empty((M, N), dtype=dtype, device=x.device)
+        out = x.new_empty((M, N))
     else:
         y_ld, one = out.stride() if out.dim() == 2 else (0, 0)
         if M < 2:
@@ -79,7 +79,7 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch
     a.y = out.data_ptr()
     if M > 16:  # fewer rows need no scratch
         need = ext.query("dsv41_gemv_w4_scratch_bytes", a)
-        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+        scratch = w.new_empty((need,))
         a.scratch, a.scratch_bytes = scratch.data_ptr(), need
     ext.call("dsv41_gemv_w4", a, stream)
     return out

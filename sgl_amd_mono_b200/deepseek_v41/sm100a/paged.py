@@ -148,7 +148,7 @@ class PagedKV:
             heads = q.shape[1]
             a.q, a.q_ld = self._rows(q, "q", rows, dtype, heads)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             a.q_out, a.q_out_ld = self._rows(q_out, "q_out", rows, dtype, heads)
         elif q_out is not None:
             raise RuntimeError("q_out without q")
@@ -174,7 +174,7 @@ class PagedKV:
         a.heads = heads
         a.q, a.q_ld = self._rows(q, "q", rows, dtype, heads)
         if out is None:
-            out = torch.empty(q.shape, dtype=dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         a.out, a.out_ld = self._rows(out, "out", rows, dtype, heads)
         if not 0 <= window < 1 << 31:
             raise RuntimeError(f"window {window}")
@@ -190,7 +190,7 @@ class PagedKV:
         need = self._scratch.get(key)
         if need is None:
             need = self._scratch[key] = ext.query("dsv41_paged_attn_scratch_bytes", a)
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        scratch = self.k.new_empty((need,))
         a.scratch, a.scratch_bytes = scratch.data_ptr(), need
         ext.call("dsv41_paged_attn", a, stream)
         return out
