@@ -9,9 +9,8 @@
 // the thread that owns the row reads back and adds to its fp32 sums times the row's scale: scales are
 // never rounded into the weights.
 //
-// 24 warps, one CTA an SM: 0 weight copies (TMA, 256 rows x 128 bytes = 256 k a stage), 1 and 6 the MMA
-// issue of the two accumulators, 2 .. 5 x, 8 .. 23 converters: two threads a row, each half of a unit's
-// k and half of the accumulator's columns. The blocks of all row tiles are cut into equal
+// 16 warps, one CTA an SM: 0 weight copies (TMA, 256 rows x 128 bytes = 256 k a stage), 1 and 6 the MMA
+// issue of the two accumulators, 2 .. 5 x, 8 .. 15 converters. The blocks of all row tiles are cut into equal
 // contiguous shares, one a CTA; tiles that lie in several shares are joined from scratch in order by
 // a second kernel.
 #pragma once
@@ -50,7 +49,7 @@ struct GemvW4TcArgs {
   float* part;         // [2 CTAs][NP][256] unfinished sums
 };
 
-constexpr int kWtThreads = 768;
+constexpr int kWtThreads = 512;
 constexpr int kWtRows = 256;
 constexpr int kWtBlock = 256;    // k a stage
 constexpr int kWtStages = 4;     // weight stages, 32 KB each
@@ -58,16 +57,19 @@ constexpr int kWtXStages = 3;
 
 template <int NP, int SUB>
 struct WtShape {
-  // accumulators of a unit: as many groups as 128 k hold, while two units' fit beside A in 256 columns
-  static constexpr int kFit = NP == 16 ? 4 : NP == 32 ? 2 : 1;
+  // accumulators of a unit: as many groups as 128 k hold and 96 columns take; two units' of them where
+  // they fit beside two units of A in a half's 256 columns, else one unit's (48 rows of x and groups of
+  // 32 or 64)
+  static constexpr int kFit = NP == 16 ? 4 : 2;
   static constexpr int kNsub = 128 / SUB < kFit ? 128 / SUB : kFit;
+  static constexpr int kDBuf = kNsub * NP <= 64 ? 2 : 1;
   static constexpr int kUnit = SUB * kNsub;  // k between two hand-overs to the tensor core
   static constexpr int kUnits = kWtBlock / kUnit;
   static constexpr int kEntries = kWtBlock / SUB;  // scales a row of a block
   static constexpr int kXStage = NP * kWtBlock * 2;
   static constexpr int kX = kWtStages * kWtRows * 128;
   static constexpr int kBar = kX + kWtXStages * kXStage;
-  static constexpr int kNumBars = 2 * kWtStages + 2 * kWtXStages + 10;
+  static constexpr int kNumBars = 2 * kWtStages + 2 * kWtXStages + 12;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kBytes = kMisc + 16 + 1024;
 };
@@ -115,24 +117,6 @@ __device__ __forceinline__ bool wt_wait(uint32_t bar, uint32_t parity, volatile 
   return false;
 }
 
-// 8 TMEM columns of this thread's lane, raw bits.
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-               : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-// Byte e of up to 8 packed bytes; e may differ between the two converters of a row, not within a warp.
-template <int EN, int W>
-__device__ __forceinline__ uint32_t sel_byte(const uint32_t (&z)[W], int e) {
-  const uint32_t v = EN > 4 && e >= 4 ? z[W - 1] : z[0];
-  return v >> (8 * (e & 3));
-}
-
 template <bool F16, int NP, int SUB>
 __global__ void __launch_bounds__(kWtThreads, 1)
     gemv_w4_tc_kernel(const __grid_constant__ CUtensorMap wmap, const GemvW4TcArgs p) {
@@ -150,15 +134,16 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   auto x_empty = [&](int s) { return bars + 8 * (2 * SW + SX + s); };
   auto a_full = [&](int h, int b) { return bars + 8 * (2 * SW + 2 * SX + 2 * h + b); };
   auto d_full = [&](int h, int b) { return bars + 8 * (2 * SW + 2 * SX + 4 + 2 * h + b); };
+  auto d_free = [&](int h) { return bars + 8 * (2 * SW + 2 * SX + 10 + h); };  // of the only accumulators
   auto drained = [&](int h) { return bars + 8 * (2 * SW + 2 * SX + 8 + h); };
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
   if (tid == 0) {
-    for (int s = 0; s < SW; ++s) mbar_init(w_full(s), 1), mbar_init(w_empty(s), 16);
+    for (int s = 0; s < SW; ++s) mbar_init(w_full(s), 1), mbar_init(w_empty(s), 8);
     for (int s = 0; s < SX; ++s) mbar_init(x_full(s), 128), mbar_init(x_empty(s), 2);
     for (int h = 0; h < 2; ++h) {
-      for (int b = 0; b < 2; ++b) mbar_init(a_full(h, b), 8), mbar_init(d_full(h, b), 1);
-      mbar_init(drained(h), 1);
+      for (int b = 0; b < 2; ++b) mbar_init(a_full(h, b), 4), mbar_init(d_full(h, b), 1);
+      mbar_init(drained(h), 1), mbar_init(d_free(h), 4);
     }
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -214,11 +199,12 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         const int nu = units(kb);
         for (int x = 0; x < nu; ++x, ++u) {
           if (!(ok = wt_wait(a_full(h, u & 1), (u >> 1) & 1, abort))) break;
+          if (L::kDBuf == 1 && u && !(ok = wt_wait(d_free(h), (u - 1) & 1, abort))) break;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < UK / 16; ++k) {
             const int kk = x * UK + 16 * k;  // 64-k chunks of NP rows, 16 k = 32 bytes into a row
-            umma_f16_ts(td + 64 * (u & 1) + (16 * k / SUB) * NP, ta + 64 * (u & 1) + 8 * k,
+            umma_f16_ts(td + (L::kDBuf == 2 ? 64 * (u & 1) : 0) + (16 * k / SUB) * NP, ta + 64 * (u & 1) + 8 * k,
                         umma_sdesc_sw128(sx + (kk >> 6) * NP * 128 + (kk & 63) * 2, 16, 1024), idesc, 16 * k % SUB != 0);
           }
           umma_commit(d_full(h, u & 1));
@@ -254,11 +240,9 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       if (++kb == p.kblocks) kb = 0;
     }
   } else if (warp >= 8) {
-    // half h of the rows, half `half` of a unit's k and of the accumulator's columns
-    const int h = ((warp - 8) >> 2) & 1, half = (warp - 8) >> 3, row = 128 * h + 32 * (warp & 3) + lane;
-    constexpr int NH = NP / 2;
+    const int h = (warp - 8) >> 2, row = 128 * h + 32 * (warp & 3) + lane;
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t ta = tmem + 256 * h + lane_base + half * (UK / 4), td = tmem + 256 * h + 128 + lane_base + half * NH;
+    const uint32_t ta = tmem + 256 * h + lane_base, td = ta + 128;
     const uint32_t wrow = smem_u32(smem) + row * 128;
     const int groups = a.K / a.group;
     const W4Consts<F16> consts;
@@ -304,9 +288,9 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         }
       }
     };
-    float acc[NH];
+    float acc[NP];
 #pragma unroll
-    for (int m = 0; m < NH; ++m) acc[m] = 0.f;
+    for (int m = 0; m < NP; ++m) acc[m] = 0.f;
     // the unit whose accumulators are not read yet: its scales, and where its tile's sums go if it is
     // the last of its tile here (0: it is not, 1: y, 2: scratch)
     float held[NS];
@@ -317,32 +301,36 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       const int v = u - 1;
       if (!__all_sync(0xffffffffu, wt_wait(d_full(h, v & 1), (v >> 1) & 1, abort))) return false;
       tc_fence_after();
-      uint32_t d[NS][NH];
 #pragma unroll
       for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int c = 0; c < NH; c += 8)
-          tmem_ld8(td + 64 * (v & 1) + s * NP + c, *reinterpret_cast<uint32_t(*)[8]>(d[s] + c));
-      tmem_wait_ld();
+        for (int c = 0; c < NP; c += 16) {
+          uint32_t d[16];
+          tmem_ld16(td + (L::kDBuf == 2 ? 64 * (v & 1) : 0) + s * NP + c, d);
+          tmem_wait_ld();
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int m = 0; m < NH; ++m) acc[m] = fmaf(__uint_as_float(d[s][m]), held[s], acc[m]);
+          for (int m = 0; m < 16; ++m) acc[c + m] = fmaf(__uint_as_float(d[m]), held[s], acc[c + m]);
+        }
+      if (L::kDBuf == 1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(d_free(h));
+      }
       if (out) {
-        const int n = out_tile * kWtRows + row, m0 = half * NH;
+        const int n = out_tile * kWtRows + row;
         if (out == 1) {
-          T* y = reinterpret_cast<T*>(a.y) + m0 * a.y_ld + n;
+          T* y = reinterpret_cast<T*>(a.y) + n;
 #pragma unroll
-          for (int m = 0; m < NH; ++m)
-            if (m0 + m < a.M && n < a.N) y[m * a.y_ld] = Act<F16>::r(acc[m]);
+          for (int m = 0; m < NP; ++m)
+            if (m < a.M && n < a.N) y[m * a.y_ld] = Act<F16>::r(acc[m]);
         } else {
-          float* y = p.part + ((int64_t)out_slot * NP + m0) * kWtRows + row;
+          float* y = p.part + (int64_t)out_slot * NP * kWtRows + row;
 #pragma unroll
-          for (int m = 0; m < NH; ++m)
-            if (m0 + m < a.M) y[m * kWtRows] = acc[m];
+          for (int m = 0; m < NP; ++m)
+            if (m < a.M) y[m * kWtRows] = acc[m];
         }
 #pragma unroll
-        for (int m = 0; m < NH; ++m) acc[m] = 0.f;
+        for (int m = 0; m < NP; ++m) acc[m] = 0.f;
       }
       return true;
     };
@@ -362,27 +350,17 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       for (int x = 0; x < L::kUnits; ++x) {
         if (x >= nu) break;
 #pragma unroll
-        for (int q = 0; q < (UK + 63) / 64; ++q) {
-          // 32 k (a 16-byte unit of the row), or 16 where a unit of the tensor core's has only 32
-          const int k = x * UK + half * (UK / 2) + 32 * q;
-          const uint32_t at = wrow + s * kWtRows * 128 + (((k >> 5) ^ (row & 7)) << 4);
-          const uint32_t z = sel_byte<EN>(ze, k / SUB) & 15u;
+        for (int q = 0; q < UK / 32; ++q) {
+          const int c = x * (UK / 32) + q, e = 32 * c / SUB;  // the row's 16-byte unit, its scale
+          const uint4 w = lds16(wrow + s * kWtRows * 128 + ((c ^ (row & 7)) << 4));
+          const uint32_t z = (ze[e / 4] >> (8 * (e & 3))) & 15u;
           const uint32_t zz = (z | z << 16) + consts.one;
-          if constexpr (UK >= 64) {
-            const uint4 w = lds16(at);
-            uint32_t r[16];
-            w4_unpack_z<F16>(consts, w.x, zz, *reinterpret_cast<uint32_t(*)[4]>(r));
-            w4_unpack_z<F16>(consts, w.y, zz, *reinterpret_cast<uint32_t(*)[4]>(r + 4));
-            w4_unpack_z<F16>(consts, w.z, zz, *reinterpret_cast<uint32_t(*)[4]>(r + 8));
-            w4_unpack_z<F16>(consts, w.w, zz, *reinterpret_cast<uint32_t(*)[4]>(r + 12));
-            tmem_st16(ta + 64 * (u & 1) + 16 * q, r);
-          } else {
-            const uint2 w = lds8(at + (k & 31) / 2);
-            uint32_t r[8];
-            w4_unpack_z<F16>(consts, w.x, zz, *reinterpret_cast<uint32_t(*)[4]>(r));
-            w4_unpack_z<F16>(consts, w.y, zz, *reinterpret_cast<uint32_t(*)[4]>(r + 4));
-            tmem_st8(ta + 64 * (u & 1), r);
-          }
+          uint32_t r[16];
+          w4_unpack_z<F16>(consts, w.x, zz, *reinterpret_cast<uint32_t(*)[4]>(r));
+          w4_unpack_z<F16>(consts, w.y, zz, *reinterpret_cast<uint32_t(*)[4]>(r + 4));
+          w4_unpack_z<F16>(consts, w.z, zz, *reinterpret_cast<uint32_t(*)[4]>(r + 8));
+          w4_unpack_z<F16>(consts, w.w, zz, *reinterpret_cast<uint32_t(*)[4]>(r + 12));
+          tmem_st16(ta + 64 * (u & 1) + 16 * q, r);
         }
         tmem_wait_st();
         tc_fence_before();
