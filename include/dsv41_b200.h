@@ -310,10 +310,11 @@ int dsv41_argmax_decode(const Dsv41ArgmaxArgs* a, void* stream);
  * y[m][n] = sum_k x[m][k] * (w[n][k] - z[n][k / group]) * s[n][k / group], summed in fp32 and
  * rounded once to x's type: w unsigned 4-bit values packed two a byte, [N, K / 2] row-major (even
  * k in the low nibble) and read in place; scales [N, K / group] of x's type; zeros u8
- * [N, K / group] (values 0 .. 15) or 0 for 8 everywhere; x [M, x_ld] and y [M, y_ld] bf16, or f16
- * with f16 = 1. M <= 48, K a multiple of group, group a multiple of 32; w and x 16-byte aligned,
- * x_ld a multiple of 8. Up to 16 rows need no scratch. No counterpart in the reference (its dense
- * projections are FP8). */
+ * [N, K / group] (values 0 .. 15) or 0 for 8 everywhere; x [M, x_ld] and y [M, y_ld] bf16 (below
+ * 2^63 in magnitude), or f16 with f16 = 1. M <= 48, K a multiple of group, group a multiple of 32;
+ * w and x 16-byte aligned, x_ld a multiple of 8. An infinity or NaN in a row of x makes that row of
+ * y not finite, one in a scale that column. Up to 16 rows need no scratch. No counterpart in the
+ * reference (its dense projections are FP8). */
 typedef struct {
   int64_t w, scales, zeros, x, y;     /* device pointers */
   int64_t M, N, K, group, x_ld, y_ld, f16;

@@ -81,10 +81,15 @@ template <bool F16>
 __device__ __forceinline__ float w4_scale() {
   return F16 ? 0x1p-24f : 0x1p-133f;
 }
-// What turns the fp32 sums into the product's: 2^24 for f16, 2^(133 - 64) for bf16.
+// What turns the fp32 sums into the product's, 2^24 for f16 and 2^(133 - 64) for bf16: half of it goes
+// into the groups' scales, the rest onto the finished sum, so that neither end leaves fp32's range.
+template <bool F16>
+__device__ __forceinline__ float w4_unscale_group() {
+  return F16 ? 0x1p12f : 0x1p35f;
+}
 template <bool F16>
 __device__ __forceinline__ float w4_unscale() {
-  return F16 ? 0x1p24f : 0x1p69f;
+  return F16 ? 0x1p12f : 0x1p34f;
 }
 
 // 16 bytes at src + o into shared memory, zeros from src + end on.
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(32 * kW4Warps) gemv_w4_kernel(const GemvW4Args
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int e = 0; e < EL; ++e) {
-        const float z = (float)(ze[r][e] & 15u), s = Act<F16>::unpack(sc[r][e]).x;
+        const float z = (float)(ze[r][e] & 15u), s = Act<F16>::unpack(sc[r][e]).x * w4_unscale_group<F16>();
         *reinterpret_cast<float2*>(p + ((e0 + e) * ROWS + 16 * r + (lane & 15)) * 8) = make_float2(-z, s);
       }
     held = -1;
@@ -297,7 +302,7 @@ __global__ void __launch_bounds__(32 * kW4Warps) gemv_w4_kernel(const GemvW4Args
             asm volatile("ld.shared.u16 %0, [%1];" : "=r"(v) : "r"(tab + 2 * at));
             if (a.zeros) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(tab + ROWS * groups * 2 + at));
             nz[r][h] = -(float)(z & 15u);
-            sc2[r][h] = Act<F16>::unpack(v).x;
+            sc2[r][h] = Act<F16>::unpack(v).x * w4_unscale_group<F16>();
           } else {
             const uint2 v = lds8(sz + (e * ROWS + 16 * r + 8 * h) * 8);
             nz[r][h] = __uint_as_float(v.x);

@@ -53,7 +53,7 @@ bool append_ok(const Dsv41KvAppendArgs* a) {
 
 bool attn_ok(const Dsv41PagedAttnArgs* a) {
   return paged_ok(a) && rows_ok(a->q, a->q_ld, a->heads, a->dim) && rows_ok(a->out, a->out_ld, a->heads, a->dim) &&
-         a->window >= 0 && a->window <= INT_MAX && a->sink % 4 == 0;
+         a->window >= 0 && a->window <= INT_MAX && a->sink % 4 == 0 && a->T * (a->heads / a->kv_heads) <= (1 << 30);
 }
 
 // Columns of 8 a CTA takes together. A sequence's columns (its rows times the query heads of a kv

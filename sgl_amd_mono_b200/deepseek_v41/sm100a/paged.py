@@ -153,7 +153,8 @@ class PagedKV:
         elif q_out is not None:
             raise RuntimeError("q_out without q")
         a.heads = heads
-        ext.call("dsv41_kv_append", a, stream)
+        if rows and a.seqs:
+            ext.call("dsv41_kv_append", a, stream)
         return q_out
 
     def attend(self, q: torch.Tensor, *, lens: torch.Tensor, table: torch.Tensor, scale: float,
@@ -184,9 +185,11 @@ class PagedKV:
                     or not sink.is_contiguous():
                 raise RuntimeError(f"sink: {tuple(sink.shape)} {sink.dtype} on {sink.device}: want [{heads}] fp32")
             a.sink = sink.data_ptr()
+        if not rows or not a.seqs:
+            return out
         a.scale_f32 = _U32.unpack(_F32.pack(scale))[0]
         # the scratch depends on the heads and on the rows a sequence has on average
-        key = heads, -(-rows // a.seqs) if a.seqs else 0
+        key = heads, -(-rows // a.seqs)
         need = self._scratch.get(key)
         if need is None:
             need = self._scratch[key] = ext.query("dsv41_paged_attn_scratch_bytes", a)

@@ -40,7 +40,7 @@ BAD_PAGED = [dict(T=-1), dict(T=1 << 30), dict(seqs=-1), dict(heads=0), dict(hea
 BAD_APPEND = [dict(k=0), dict(v=0), dict(k=P + 2), dict(v_ld=120), dict(k_ld=132), dict(q_out=0), dict(q_out=P + 2),
               dict(q_out_ld=500), dict(rope=-16), dict(rope=80), dict(rope=24), dict(neox=2), dict(cos_sin=0),
               dict(cos_sin=P + 4), dict(rope_rows=0)]
-BAD_ATTN = [dict(q=0), dict(out=0), dict(out=P + 2), dict(out_ld=504), dict(window=-1), dict(window=1 << 31),
+BAD_ATTN = [dict(T=1 << 24, heads=1024, q_ld=1 << 20, out_ld=1 << 20), dict(q=0), dict(out=0), dict(out=P + 2), dict(out_ld=504), dict(window=-1), dict(window=1 << 31),
             dict(sink=P + 2)]
 
 
