@@ -82,22 +82,25 @@ int64_t attn_go(const Dsv41PagedAttnArgs* a, F f) {
   return a->dim == 64 ? by_tiles(Int<64>()) : a->dim == 128 ? by_tiles(Int<128>()) : by_tiles(Int<256>());
 }
 
+// As many CTAs as fit the GPU, or as there can be units of work in the pages that the table can name.
 template <int D, int NT>
-int64_t attn_ctas() {
-  return (int64_t)device_sms() * PaShape<D, NT>::kCtas;
+int64_t attn_ctas(const Dsv41PagedAttnArgs* a) {
+  const int64_t cts = a->T * (a->heads / a->kv_heads) / (8 * NT) + a->seqs;
+  const int64_t steps = cdiv64(a->width * a->page / 16 + 1, PaShape<D, NT>::kWarps);
+  return std::min((int64_t)device_sms() * PaShape<D, NT>::kCtas, std::max<int64_t>(1, cts * a->kv_heads * steps));
 }
 template <int D, int NT>
-int64_t attn_scratch() {
-  return attn_ctas<D, NT>() * (2 * 8 * NT * (D * sizeof(float) + sizeof(float4)) + sizeof(PaSplit));
+int64_t attn_scratch(const Dsv41PagedAttnArgs* a) {
+  return attn_ctas<D, NT>(a) * (2 * 8 * NT * (D * sizeof(float) + sizeof(float4)) + sizeof(PaSplit));
 }
 
 template <int F16, int D, int NT>
 int attn_run(const Dsv41PagedAttnArgs* a, void* stream) {
-  if (!a->scratch || a->scratch % 16 || a->scratch_bytes < attn_scratch<D, NT>()) return DSV41_ESCRATCH;
+  if (!a->scratch || a->scratch % 16 || a->scratch_bytes < attn_scratch<D, NT>(a)) return DSV41_ESCRATCH;
   const uint32_t bits = (uint32_t)a->scale_f32;
   float scale;
   memcpy(&scale, &bits, 4);
-  const int64_t ctas = attn_ctas<D, NT>(), slots = 2 * ctas * 8 * NT;
+  const int64_t ctas = attn_ctas<D, NT>(a), slots = 2 * ctas * 8 * NT;
   float* part = ptr<float>(a->scratch);
   const PagedAttnArgs p = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->window, scale * 1.44269504f,
                            ptr<const void>(a->q), ptr<void>(a->out), a->q_ld, a->out_ld, ptr<const float>(a->sink),
@@ -141,7 +144,7 @@ int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
 
 int64_t dsv41_paged_attn_scratch_bytes(const Dsv41PagedAttnArgs* a) {
   if (!attn_ok(a)) return DSV41_EINVAL;
-  return attn_go(a, [](auto, auto d, auto nt) { return attn_scratch<d, nt>(); });
+  return attn_go(a, [&](auto, auto d, auto nt) { return attn_scratch<d, nt>(a); });
 }
 
 int dsv41_paged_attn(const Dsv41PagedAttnArgs* a, void* stream) {

@@ -8,8 +8,8 @@
 //
 // The work is copying, so everything moves 16 bytes a lane at a time in units of 16 dims: two 8-dim
 // pieces that hold 8 whole rotation pairs and share 8 angles, side by side for pairs (2j, 2j + 1) and
-// half a rotation apart for (j, j + rope / 2). A block's rows are read twice, for the largest magnitude
-// and to be written; the second time from L1.
+// half a rotation apart for (j, j + rope / 2). A block's rows are looked at twice, for the largest
+// magnitude and to be written, the first 16 (of 128 dims) in registers and what is more from L1.
 #pragma once
 
 #include "gqa.cuh"
@@ -42,10 +42,8 @@ __device__ __forceinline__ RopeUnit rope_unit(int u, int dim, int rope, int neox
   return {16 * u, 16 * u + 8, ur >= 0 ? 8 * ur : -1};
 }
 
-// (A plain load: the queries may be rotated in place.)
 template <bool F16>
-__device__ __forceinline__ void load8(const typename Act<F16>::T* x, float* v) {
-  const uint4 w = *reinterpret_cast<const uint4*>(x);
+__device__ __forceinline__ void unpack8(uint4 w, float* v) {
   const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -104,23 +102,42 @@ __device__ __forceinline__ void append_block(const KvAppendArgs& a, int seq, int
   const int rope = is_k ? a.rope : 0;
   const RopeUnit ru = rope_unit(lane % UNITS, D, rope, a.neox);
   const int old = in ? *cp : 0;
-  auto value = [&](int i, float (&v)[16]) {
+  // the lane's units of rows i, i + PER, ..: KEEP of them stay in registers for the second pass (all of a
+  // block of 16 up to 128 dims)
+  constexpr int KEEP = 4;
+  auto load = [&](int i, uint4 (&w)[2]) {
     const T* row = x + (r + i) * ld;
-    load8<F16>(row + ru.d0, v);
-    load8<F16>(row + ru.d1, v + 8);
+    w[0] = ldg16(row + ru.d0);
+    w[1] = ldg16(row + ru.d1);
+  };
+  auto value = [&](int i, const uint4 (&w)[2], float (&v)[16]) {
+    unpack8<F16>(w[0], v);
+    unpack8<F16>(w[1], v + 8);
     if (rope && ru.angle >= 0) {
       Angles an;
       load_angles(a.cos_sin + rope_row(pos + i, a.rope_rows) * rope, rope, ru.angle, an);
       rotate16(v, an, a.neox);
     }
   };
+  const int i0 = lane / UNITS;
+  uint4 kept[KEEP][2];
+#pragma unroll
+  for (int n = 0; n < KEEP; ++n)
+    if (i0 + n * PER < rows) load(i0 + n * PER, kept[n]);
   float amax = 0.f;
-#pragma unroll 2
-  for (int i = lane / UNITS; i < rows; i += PER) {
+  auto see = [&](int i, const uint4 (&w)[2]) {
     float v[16];
-    value(i, v);
+    value(i, w, v);
 #pragma unroll
     for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(v[e]));  // NaN does not count
+  };
+#pragma unroll
+  for (int n = 0; n < KEEP; ++n)
+    if (i0 + n * PER < rows) see(i0 + n * PER, kept[n]);
+  for (int i = i0 + KEEP * PER; i < rows; i += PER) {
+    uint4 w[2];
+    load(i, w);
+    see(i, w);
   }
   amax = fminf(warp_max(amax), 3.402823466e38f);
   int code = code_ceil(__fdiv_rn(fmaxf(amax, 1e-4f), kFp8Max));
@@ -138,16 +155,23 @@ __device__ __forceinline__ void append_block(const KvAppendArgs& a, int seq, int
     }
   }
   const float mul = mx_mul(code);
-#pragma unroll 2
-  for (int i = lane / UNITS; i < rows; i += PER) {
+  auto put = [&](int i, const uint4 (&x)[2]) {
     float v[16];
-    value(i, v);
+    value(i, x, v);
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = e4m3x4(v[4 * e] * mul, v[4 * e + 1] * mul, v[4 * e + 2] * mul, v[4 * e + 3] * mul);
     uint8_t* y = dst + (in + i) * D;
     *reinterpret_cast<uint2*>(y + ru.d0) = make_uint2(w[0], w[1]);
     *reinterpret_cast<uint2*>(y + ru.d1) = make_uint2(w[2], w[3]);
+  };
+#pragma unroll
+  for (int n = 0; n < KEEP; ++n)
+    if (i0 + n * PER < rows) put(i0 + n * PER, kept[n]);
+  for (int i = i0 + KEEP * PER; i < rows; i += PER) {
+    uint4 w[2];
+    load(i, w);
+    put(i, w);
   }
   __syncwarp();
   if (lane == 0) *cp = (uint8_t)code;
@@ -215,19 +239,29 @@ __global__ void __launch_bounds__(kApThreads) kv_append_kernel(const KvAppendArg
   }
   const T* x = reinterpret_cast<const T*>(a.q) + row * a.q_ld;
   T* y = reinterpret_cast<T*>(a.q_out) + row * a.q_out_ld;
-  const int h1 = min(h0 + a.head_step, a.heads);
-#pragma unroll 4
-  for (int h = h0; h < h1; ++h) {
-    float v[16];
-    load8<F16>(x + h * D + ru.d0, v);
-    load8<F16>(x + h * D + ru.d1, v + 8);
-    if (a.rope && ru.angle >= 0) rotate16(v, an, a.neox);
-    uint32_t w[8];
+  // every load ahead of the first store (plain loads: the queries may be rotated in place, a thread's own
+  // values each)
+  constexpr int HEADS = 4;
+  uint4 in[HEADS][2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = Act<F16>::pack(v[2 * e], v[2 * e + 1]);
-    *reinterpret_cast<uint4*>(y + h * D + ru.d0) = make_uint4(w[0], w[1], w[2], w[3]);
-    *reinterpret_cast<uint4*>(y + h * D + ru.d1) = make_uint4(w[4], w[5], w[6], w[7]);
-  }
+  for (int n = 0; n < HEADS; ++n)
+    if (n < a.head_step && h0 + n < a.heads) {
+      in[n][0] = *reinterpret_cast<const uint4*>(x + (h0 + n) * D + ru.d0);
+      in[n][1] = *reinterpret_cast<const uint4*>(x + (h0 + n) * D + ru.d1);
+    }
+#pragma unroll
+  for (int n = 0; n < HEADS; ++n)
+    if (n < a.head_step && h0 + n < a.heads) {
+      float v[16];
+      unpack8<F16>(in[n][0], v);
+      unpack8<F16>(in[n][1], v + 8);
+      if (a.rope && ru.angle >= 0) rotate16(v, an, a.neox);
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = Act<F16>::pack(v[2 * e], v[2 * e + 1]);
+      *reinterpret_cast<uint4*>(y + (h0 + n) * D + ru.d0) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(y + (h0 + n) * D + ru.d1) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
 }
 
 }  // namespace dsv41

@@ -51,7 +51,6 @@ class PagedKV:
         self.k, self.v, self.k_codes, self.v_codes = k, v, k_codes, v_codes
         self.pages, self.kv_heads, self.page, self.dim, self.block = pages, heads, page, dim, page // per
         self._dev = k.get_device()
-        self._scratch: dict = {}  # attention's scratch bytes by (heads, rows a sequence)
         cache = dict(kv_heads=heads, dim=dim, k_cache=k.data_ptr(), v_cache=v.data_ptr(), k_codes=k_codes.data_ptr(),
                      v_codes=v_codes.data_ptr(), pages=pages, page=page, block=self.block)
         self._append_args, self._attend_args = bytes(abi.KvAppendArgs(**cache)), bytes(abi.PagedAttnArgs(**cache))
@@ -188,11 +187,7 @@ class PagedKV:
         if not rows or not a.seqs:
             return out
         a.scale_f32 = _U32.unpack(_F32.pack(scale))[0]
-        # the scratch depends on the heads and on the rows a sequence has on average
-        key = heads, -(-rows // a.seqs)
-        need = self._scratch.get(key)
-        if need is None:
-            need = self._scratch[key] = ext.query("dsv41_paged_attn_scratch_bytes", a)
+        need = ext.query("dsv41_paged_attn_scratch_bytes", a)
         scratch = self.k.new_empty((need,))
         a.scratch, a.scratch_bytes = scratch.data_ptr(), need
         ext.call("dsv41_paged_attn", a, stream)
