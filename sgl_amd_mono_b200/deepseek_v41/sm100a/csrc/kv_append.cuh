@@ -9,7 +9,7 @@
 // The work is copying, so everything moves 16 bytes a lane at a time in units of 16 dims: two 8-dim
 // pieces that hold 8 whole rotation pairs and share 8 angles, side by side for pairs (2j, 2j + 1) and
 // half a rotation apart for (j, j + rope / 2). A block's rows are looked at twice, for the largest
-// magnitude and to be written, the first 16 (of 128 dims) in registers and what is more from L1.
+// magnitude and to be written, some of them in registers and the others from L1.
 #pragma once
 
 #include "gqa.cuh"
@@ -102,9 +102,9 @@ __device__ __forceinline__ void append_block(const KvAppendArgs& a, int seq, int
   const int rope = is_k ? a.rope : 0;
   const RopeUnit ru = rope_unit(lane % UNITS, D, rope, a.neox);
   const int old = in ? *cp : 0;
-  // the lane's units of rows i, i + PER, ..: KEEP of them stay in registers for the second pass (all of a
-  // block of 16 up to 128 dims)
-  constexpr int KEEP = 4;
+  // the lane's units of rows i, i + PER, ..: KEEP of them stay in registers for the second pass (4 keep all
+  // of a block of 16 rows of 128 dims, but with 2 four CTAs fit an SM: ragged prompts 53 us against 59)
+  constexpr int KEEP = 2;
   auto load = [&](int i, uint4 (&w)[2]) {
     const T* row = x + (r + i) * ld;
     w[0] = ldg16(row + ru.d0);
@@ -192,7 +192,7 @@ __device__ __forceinline__ int row_seq_search(const StepRows& s, int r) {
 // CTAs [0, kv_ctas): a warp a (window of rows, key or value head); the others: a thread a (row, head_step
 // query heads, unit).
 template <bool F16, int D>
-__global__ void __launch_bounds__(kApThreads) kv_append_kernel(const KvAppendArgs a) {
+__global__ void __launch_bounds__(kApThreads, 4) kv_append_kernel(const KvAppendArgs a) {
   using T = typename Act<F16>::T;
   constexpr int UNITS = D / 16;
   pdl_wait();
