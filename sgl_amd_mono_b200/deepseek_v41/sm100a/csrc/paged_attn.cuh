@@ -171,6 +171,12 @@ __device__ __forceinline__ void pa_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// {lo, hi} rounded to f16x2 by one instruction.
+__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 template <class V>
 __device__ __forceinline__ V pa_lds(const uint8_t* p) {
   return *reinterpret_cast<const V*>(p);
@@ -181,11 +187,11 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w &
 template <int D, int NT>
 struct PaShape {
   // What a thread holds decides how many warps an SM runs: two CTAs of 8 while O takes up to 32 registers
-  // (and the fragments of Q as many), one of 12 up to 96, else one of 8 (8 sequences of 4 rows and 4 heads
-  // a kv head at 32768 tokens, O of 64: 121 us with 12 warps, 125 with two CTAs of 8, 140 with 8).
+  // (and the fragments of Q as many), one of 12 up to 64, else one of 8 (8 sequences at 32768 tokens: O of
+  // 64 121 us with 12 warps, 125 with two CTAs of 8, 140 with 8; O of 96 192 us with 12 and 154 with 8).
   static constexpr int kO = NT * D / 4;               // O registers a thread
   static constexpr int kCtas = kO <= 32 ? 2 : 1;      // an SM
-  static constexpr int kWarps = kO <= 32 || kO > 96 ? 8 : 12;
+  static constexpr int kWarps = kO <= 32 || kO > 64 ? 8 : 12;
   static constexpr int kTile = 32 * D;                // bytes of a staged tile, K and V
   static constexpr int kStagesFit = 192 / kCtas * 1024 / (kWarps * kTile);
   static constexpr int kStages = kStagesFit > 6 ? 6 : kStagesFit;
@@ -193,7 +199,8 @@ struct PaShape {
   static constexpr int kRing = kWarps * kStages * kTile;
   static constexpr int kQBytes = kQSmem ? 8 * NT * D * 2 : 0;
   static constexpr int kRl = kWarps * 8 * NT * 16;    // the warps' references and sums
-  static constexpr int kBytes = kRing + kQBytes + kRl + (kWarps + 2) * 8;
+  static constexpr int kSc = kWarps * kStages * 8;    // a staged tile's scales
+  static constexpr int kBytes = kRing + kQBytes + kRl + kSc + (kWarps + 2) * 8;
   static_assert(kWarps / 2 * 8 * NT * D * 4 <= kRing, "the merge reuses the ring");
 };
 
@@ -217,7 +224,8 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
   extern __shared__ __align__(128) uint8_t pa_smem[];
   uint2* q_sm = reinterpret_cast<uint2*>(pa_smem + P::kRing);
   float4* rl_sm = reinterpret_cast<float4*>(pa_smem + P::kRing + P::kQBytes);
-  long long* plan_sm = reinterpret_cast<long long*>(pa_smem + P::kRing + P::kQBytes + P::kRl);
+  float2* sc_sm = reinterpret_cast<float2*>(pa_smem + P::kRing + P::kQBytes + P::kRl) + (threadIdx.x >> 5) * S;
+  long long* plan_sm = reinterpret_cast<long long*>(pa_smem + P::kRing + P::kQBytes + P::kRl + P::kSc);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring_p = pa_smem + warp * S * P::kTile;
   const uint32_t ring = smem_u32(ring_p);
@@ -336,54 +344,62 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
     // the warp's tiles: w.tile0 + first + W j, j < count
     const int first = step0 * W + warp;
     const int count = max(0, (min(step1 * W, w.tiles) - first + W - 1) / W);
-    // lane i holds page and scale codes of tile 32 b + i of the batch being issued (cur) and of the
-    // one before (prev): page, or -1 where the piece sees none of the tile's tokens
-    int cur_pg = -1, prev_pg = -1;
-    uint32_t cur_sc = 0, prev_sc = 0;
+    // lane i holds of tile 32 b + i of the batch b being issued where its keys begin in the cache, or -1 where
+    // the piece sees none of its tokens, and its scales (the keys' power of two, the values' exponent), which
+    // it leaves beside the staged tile. The divisions by the page and the block are made here, once a tile by
+    // one lane.
+    int64_t bat_at = -1;
+    float2 bat_sc = make_float2(0.f, 0.f);
     const int tile_first = w.tile0 + first;
     auto load_batch = [&](int b) {
-      prev_pg = cur_pg, prev_sc = cur_sc;
       const int j = 32 * b + lane, p0 = (tile_first + W * j) * 16;
-      cur_pg = -1;
+      bat_at = -1;
+      bat_sc.x = 0.f;  // no tile
       if (j < count && p0 < any_hi && p0 + 16 > any_lo) {
-        cur_pg = token_page(a.rows, a.cache, seq, p0);
-        if (cur_pg >= 0) {
-          const int64_t ci = ((int64_t)cur_pg * kvh + hk) * (page / block) + p0 % page / block;
-          cur_sc = a.cache.k_codes[ci] | ((uint32_t)a.cache.v_codes[ci] << 8);
+        const int pg = token_page(a.rows, a.cache, seq, p0);
+        if (pg >= 0) {
+          const int off = p0 % page;
+          const int64_t head = (int64_t)pg * kvh + hk, ci = head * (page / block) + off / block;
+          bat_at = (head * page + off) * D;
+          bat_sc = make_float2(pow2c(a.cache.k_codes[ci]), (float)((int)a.cache.v_codes[ci] - 127));
         }
       }
     };
+    const uint32_t lane_dst = ring + pa_chunk<D>(lane / (D / 16), lane % (D / 16));
+    int is_st = 0;  // the stage to issue into
     auto issue = [&](int j) {
       if (j < count) {
         if (j % 32 == 0) load_batch(j / 32);
-        const int pg = __shfl_sync(0xffffffffu, cur_pg, j & 31);
-        if (pg >= 0) {
-          const int64_t at = (((int64_t)pg * kvh + hk) * page + (tile_first + W * j) * 16 % page) * D;
-          const uint32_t dst = ring + j % S * P::kTile;
+        const int64_t at = __shfl_sync(0xffffffffu, bat_at, j & 31);
+        if (lane == (j & 31)) sc_sm[is_st] = bat_sc;
+        if (at >= 0) {
+          const uint8_t *ks = a.cache.k + at + lane * 16, *vs = a.cache.v + at + lane * 16;
+          const uint32_t dst = is_st * P::kTile;
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) {
-            const int idx = lane + 32 * i;
-            const uint32_t d = dst + pa_chunk<D>(idx / (D / 16), idx % (D / 16));
-            cp_async16_stream(d, a.cache.k + at + idx * 16);
-            cp_async16_stream(d + 16 * D, a.cache.v + at + idx * 16);
+            // 32 pieces on are 512 / D rows on: so many units further round the swizzle
+            const uint32_t d = (lane_dst ^ (D == 64 ? 0 : (512 / D * i & 7) << 4)) + dst + i * 512;
+            cp_async16_stream(d, ks + i * 512);
+            cp_async16_stream(d + 16 * D, vs + i * 512);
           }
         }
+        is_st = is_st == S - 1 ? 0 : is_st + 1;
       }
       cp_async_commit();
     };
 #pragma unroll 1
     for (int j = 0; j < S - 1; ++j) issue(j);
+    int rd_st = 0;  // the stage to read
 #pragma unroll 1
     for (int j = 0; j < count; ++j) {
       issue(j + S - 1);
       cp_async_wait<S - 1>();
       __syncwarp();
-      // batch j / 32 is cur, or prev once the issue has gone on to the next
-      const bool is_cur = min(j + S - 1, count - 1) / 32 == j / 32;
-      const int pg = __shfl_sync(0xffffffffu, is_cur ? cur_pg : prev_pg, j & 31);
-      const uint32_t sc = __shfl_sync(0xffffffffu, is_cur ? cur_sc : prev_sc, j & 31);
-      if (pg < 0) continue;
-      const uint8_t *kt = ring_p + j % S * P::kTile, *vt = kt + 16 * D;
+      const uint8_t *kt = ring_p + rd_st * P::kTile, *vt = kt + 16 * D;
+      const float2 sc = sc_sm[rd_st];
+      rd_st = rd_st == S - 1 ? 0 : rd_st + 1;
+      if (sc.x == 0.f) continue;
+      const float ks = sc.x, ev = sc.y;
       const int p0 = (tile_first + W * j) * 16;
       const bool edge = p0 < all_lo || p0 + 16 > all_hi;
 
@@ -425,8 +441,6 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
           for (int e = 0; e < 4; ++e) s[n][e] += sq[x][n][e];
 
       // s: scores, base 2; elements (token kappa, column 2t), (kappa, 2t + 1), (kappa + 8, ..)
-      const float ks = pow2c(sc & 255), ev = (float)((int)(sc >> 8) - 127);
-      bool over = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -443,11 +457,14 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
             if (p + 8 >= hi || p + 8 < lo) s[n][e + 2] = -INFINITY;
           }
       }
+      // how far the scores lie above where the references stand (at most 2^8 and 2^60 are let pass)
+      float far = -INFINITY;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) over |= s[n][e] > fminf(ref[n][e & 1] + (8.f - ev), top[n][e & 1] + 60.f);
-      if (__any_sync(0xffffffffu, over)) {
+        for (int e = 0; e < 2; ++e)
+          far = fmaxf(far, fmaxf(s[n][e], s[n][e + 2]) - fminf(ref[n][e] + (8.f - ev), top[n][e] + 60.f));
+      if (__any_sync(0xffffffffu, far > 0.f)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -471,8 +488,8 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
         for (int e = 0; e < 2; ++e) l[n][e] += ex2(s[n][e] - top[n][e]) + ex2(s[n][e + 2] - top[n][e]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] = ex2(s[n][e] + (ev + 7.f - ref[n][e & 1]));
-        pb[n][0] = movmatrix(pack_f16x2(s[n][0], s[n][1]));
-        pb[n][1] = movmatrix(pack_f16x2(s[n][2], s[n][3]));
+        pb[n][0] = movmatrix(pa_pack(s[n][0], s[n][1]));
+        pb[n][1] = movmatrix(pa_pack(s[n][2], s[n][3]));
       }
 
       // O^T += V^T P^T: lane (g, t) reads tokens t, 7 - t, t + 8, 15 - t (kappa of the mma's k = 2t,
