@@ -82,33 +82,46 @@ int64_t attn_go(const Dsv41PagedAttnArgs* a, F f) {
   return a->dim == 64 ? by_tiles(Int<64>()) : a->dim == 128 ? by_tiles(Int<128>()) : by_tiles(Int<256>());
 }
 
-// As many CTAs as fit the GPU, or as there can be units of work in the pages that the table can name.
+// How the work is cut, from what the host knows: the pages that the table can name bound the steps of a
+// sequence. Short items stay whole where each can have a CTA: one launch, no scratch. Else the GPU's CTAs
+// share all steps, no more of them than there can be, and a second launch joins the pieces. Whole against
+// split, us of GPU time, dim 128: 1 row of 4 kv heads at 120 tokens 6.4 to 7.6, 380: 7.7 to 8.7, 777: 10.1
+// to 9.3; 8 rows of 8 kv heads at 777: 10.8 to 15.6; a launch less to issue besides (10.8 us a call to 15.7
+// at 777), so 8 steps (1024 tokens) where a step is cheap. With more columns or dim 256 a step costs more (4
+// rows of 4 kv heads, groups of 8, 250 tokens: 15.5 to 16.3, 500: 18.3 to 16.2; dim 256, 250: 13.0 to
+// 14.2, 500: 15.9 to 15.0): 2 steps.
+struct AttnPlan {
+  int64_t ctas, scratch;
+  bool whole;
+};
 template <int D, int NT>
-int64_t attn_ctas(const Dsv41PagedAttnArgs* a) {
-  const int64_t cts = a->T * (a->heads / a->kv_heads) / (8 * NT) + a->seqs;
+AttnPlan attn_plan(const Dsv41PagedAttnArgs* a) {
+  const int64_t items = (a->T * (a->heads / a->kv_heads) / (8 * NT) + a->seqs) * a->kv_heads;
   const int64_t steps = cdiv64(a->width * a->page / 16 + 1, PaShape<D, NT>::kWarps);
-  return std::min((int64_t)device_sms() * PaShape<D, NT>::kCtas, std::max<int64_t>(1, cts * a->kv_heads * steps));
-}
-template <int D, int NT>
-int64_t attn_scratch(const Dsv41PagedAttnArgs* a) {
-  return attn_ctas<D, NT>(a) * (2 * 8 * NT * (D * sizeof(float) + sizeof(float4)) + sizeof(PaSplit));
+  const int64_t fit = (int64_t)device_sms() * PaShape<D, NT>::kCtas;
+  if (steps <= (PaShape<D, NT>::kO <= 32 ? 8 : 2) && items <= fit) return {std::max<int64_t>(1, items), 0, true};
+  const int64_t ctas = std::min(fit, std::max<int64_t>(1, items * steps));
+  return {ctas, ctas * (int64_t)(2 * 8 * NT * (D * sizeof(float) + sizeof(float4)) + sizeof(PaSplit)), false};
 }
 
 template <int F16, int D, int NT>
 int attn_run(const Dsv41PagedAttnArgs* a, void* stream) {
-  if (!a->scratch || a->scratch % 16 || a->scratch_bytes < attn_scratch<D, NT>(a)) return DSV41_ESCRATCH;
+  const AttnPlan plan = attn_plan<D, NT>(a);
+  if (plan.scratch && (!a->scratch || a->scratch % 16 || a->scratch_bytes < plan.scratch)) return DSV41_ESCRATCH;
   const uint32_t bits = (uint32_t)a->scale_f32;
   float scale;
   memcpy(&scale, &bits, 4);
-  const int64_t ctas = attn_ctas<D, NT>(a), slots = 2 * ctas * 8 * NT;
+  const int64_t slots = 2 * plan.ctas * 8 * NT;
   float* part = ptr<float>(a->scratch);
-  const PagedAttnArgs p = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->window, scale * 1.44269504f,
+  const PagedAttnArgs p = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->window, plan.whole, scale * 1.44269504f,
                            ptr<const void>(a->q), ptr<void>(a->out), a->q_ld, a->out_ld, ptr<const float>(a->sink),
                            part, reinterpret_cast<float4*>(part + slots * D),
                            reinterpret_cast<PaSplit*>(part + slots * (D + 4))};
-  const int rc = launch(paged_attn_kernel<F16, D, NT>, dim3((unsigned)ctas), dim3(32 * PaShape<D, NT>::kWarps),
-                        PaShape<D, NT>::kBytes, stream, p);
-  return rc ? rc : launch(paged_join_kernel<F16, D, NT>, dim3((unsigned)ctas, 8 * NT), dim3(kPaJoinThreads), 0, stream, p);
+  const dim3 grid((unsigned)plan.ctas);
+  const int rc = launch(paged_attn_kernel<F16, D, NT>, grid, dim3(32 * PaShape<D, NT>::kWarps), PaShape<D, NT>::kBytes,
+                        stream, p);
+  if (rc || plan.whole) return rc;
+  return launch(paged_join_kernel<F16, D, NT>, dim3(grid.x, 8 * NT), dim3(kPaJoinThreads), 0, stream, p);
 }
 
 }  // namespace
@@ -144,7 +157,7 @@ int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
 
 int64_t dsv41_paged_attn_scratch_bytes(const Dsv41PagedAttnArgs* a) {
   if (!attn_ok(a)) return DSV41_EINVAL;
-  return attn_go(a, [&](auto, auto d, auto nt) { return attn_scratch<d, nt>(a); });
+  return attn_go(a, [&](auto, auto d, auto nt) { return attn_plan<d, nt>(a).scratch; });
 }
 
 int dsv41_paged_attn(const Dsv41PagedAttnArgs* a, void* stream) {

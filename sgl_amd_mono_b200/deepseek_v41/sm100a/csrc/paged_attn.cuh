@@ -23,7 +23,8 @@
 // Split. The work (sequence, kv head, column tile, steps of 16 W tokens) is cut into equal
 // contiguous shares, one a CTA, whatever the lengths: each CTA finds its own from the lengths on the
 // device. A share's piece of an item that lies in several shares goes to scratch, and a second kernel
-// joins the pieces in order, so the sums do not depend on timing.
+// joins the pieces in order, so the sums do not depend on timing. Where the pages can hold only short
+// sequences and every item has a CTA, items are not split and one launch does.
 #pragma once
 
 #include <cfloat>
@@ -36,6 +37,7 @@ struct PagedAttnArgs {
   StepRows rows;
   KvCache cache;
   int heads, window;
+  int whole;    // items are not split: short sequences, no scratch and no second kernel
   float scale;  // times log2 e
   const void* q;
   void* out;
@@ -73,7 +75,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
   w.tile0 = lo / 16;
   w.tiles = max(0, (hi + 15) / 16 - w.tile0);
   w.steps = max(1, (w.tiles + W - 1) / W);
-  w.units = (long long)w.cts * kvh * w.steps;
+  w.units = (long long)w.cts * kvh * (a.whole ? 1 : w.steps);
   return w;
 }
 
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
 
   pdl_wait();
   pdl_launch();
-  if (tid == 0) a.split[blockIdx.x].pieces = 0;
+  if (tid == 0 && !a.whole) a.split[blockIdx.x].pieces = 0;
   const Share sh = find_share<NT, W>(a, blockIdx.x, gridDim.x, plan_sm);
   if (sh.seq < 0) return;
   // Where the share stands lies in shared memory between pieces, not in registers: the sequence, the
@@ -252,8 +254,8 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
       w = seq_work<NT, W>(a, ++seq);
     }
     // this piece: kv head hk, column tile ct, steps [step0, step1)
-    const int item = (int)(at / w.steps), step0 = (int)(at % w.steps);
-    const int step1 = (int)min((long long)w.steps, step0 + left);
+    const int item = (int)(a.whole ? at : at / w.steps), step0 = a.whole ? 0 : (int)(at % w.steps);
+    const int step1 = a.whole ? w.steps : (int)min((long long)w.steps, step0 + left);
     const int ct = item % w.cts, hk = item / w.cts;
     const int col0 = ct * 8 * NT;
     // what its first and last row see
@@ -664,7 +666,8 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
             }
           }
         }
-    if (tid == 0) plan_sm[0] = seq, plan_sm[1] = at + (step1 - step0), plan_sm[2] = left - (step1 - step0);
+    const int used = a.whole ? 1 : step1 - step0;
+    if (tid == 0) plan_sm[0] = seq, plan_sm[1] = at + used, plan_sm[2] = left - used;
   }
 }
 

@@ -188,7 +188,8 @@ class PagedKV:
             return out
         a.scale_f32 = _U32.unpack(_F32.pack(scale))[0]
         need = ext.query("dsv41_paged_attn_scratch_bytes", a)
-        scratch = self.k.new_empty((need,))
-        a.scratch, a.scratch_bytes = scratch.data_ptr(), need
+        if need:
+            scratch = self.k.new_empty((need,))
+            a.scratch, a.scratch_bytes = scratch.data_ptr(), need
         ext.call("dsv41_paged_attn", a, stream)
         return out

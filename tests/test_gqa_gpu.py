@@ -276,16 +276,23 @@ def run_attend(st, window=0, sink=False, scale=None):
     q = st.split(st.qkv)[0]
     qd = st.split(st.qkv.cuda())[0]
     out = torch.full((T, st.heads, st.dim), 5.0, dtype=st.dt, device="cuda")
-    got = kv.attend(qd, scale=scale, window=window, sink=None if sk is None else sk.cuda(), out=out, **st.where())
+    sk_d, where = None if sk is None else sk.cuda(), st.where()
+    got = kv.attend(qd, scale=scale, window=window, sink=sk_d, out=out, **where)
     assert got is out
     ref, sizes = G.attend(q, st.k, st.v, st.kc, st.vc, st.cu, st.lens, st.table, scale, window, sk)
     used = sum(st.rows)
-    g = out.cpu().double()
-    assert bool((g[used:] == 5.0).all()), "rows behind the last sequence moved"
-    err, tol = (g - ref).abs()[:used], attn_tol(st.dt, ref, sizes)[:used]
-    nan = ref[:used].isnan()
-    assert torch.equal(g[:used].isnan(), nan)
-    assert bool((err <= tol)[~nan].all()), (err / tol.clamp_min(1e-30))[~nan].max().item()
+    # a table with room for long sequences: the same rows, their work split and joined
+    wide = torch.full((len(st.rows), 4000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :st.table.shape[1]] = where["table"]
+    split = torch.full_like(out, 5.0)
+    kv.attend(qd, scale=scale, window=window, sink=sk_d, out=split, **{**where, "table": wide})
+    for o in (out, split):
+        g = o.cpu().double()
+        assert bool((g[used:] == 5.0).all()), "rows behind the last sequence moved"
+        err, tol = (g - ref).abs()[:used], attn_tol(st.dt, ref, sizes)[:used]
+        nan = ref[:used].isnan()
+        assert torch.equal(g[:used].isnan(), nan)
+        assert bool((err <= tol)[~nan].all()), (err / tol.clamp_min(1e-30))[~nan].max().item()
     return out
 
 

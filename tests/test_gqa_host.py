@@ -74,8 +74,11 @@ def test_paged_attn_refuses(bad):
 def test_scratch_that_does_not_do_is_refused(short):
     from sgl_amd_mono_b200.common import ext
     from sgl_amd_mono_b200.deepseek_v41.sm100a import abi
-    a = abi.PagedAttnArgs(**{**ATTN, **short})
-    assert _call("dsv41_paged_attn", a) == -3
+    long = {**ATTN, "width": 1000, "table_ld": 1000}
+    assert ext.query("dsv41_paged_attn_scratch_bytes", abi.PagedAttnArgs(**ATTN)) == 0
+    assert ext.query("dsv41_paged_attn_scratch_bytes", abi.PagedAttnArgs(**long)) > 0
+    assert _call("dsv41_paged_attn", abi.PagedAttnArgs(**{**long, **short})) == -3
+    assert ext.query("dsv41_gemv_w4_scratch_bytes", abi.GemvW4Args(**{**W4, "M": 8})) == 0
     big = {**W4, "M": 48, "N": 8192, "K": 4096, "x_ld": 4096, "y_ld": 8192}
     assert ext.query("dsv41_gemv_w4_scratch_bytes", abi.GemvW4Args(**big)) > 0
     assert _call("dsv41_gemv_w4", abi.GemvW4Args(**{**big, **short})) == -3
