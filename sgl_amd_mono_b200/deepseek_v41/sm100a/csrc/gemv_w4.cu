@@ -70,8 +70,13 @@ int w4_group(int64_t f16, const GemvW4Args& g, void* stream) {
 // ------------------------------------------------ the tcgen05 kernel
 int w4_tc_rows(const Dsv41GemvW4Args* a) { return a->M <= 16 ? 16 : a->M <= 32 ? 32 : 48; }
 // More than 16 rows over a matrix large enough to fill its pipeline (48 rows, K 4096: N 8192 28 us on
-// mma.sync and 25 here, N 28672 93 and 45; 4096 x 1024 stays at half the time on mma.sync).
-bool w4_tc(const Dsv41GemvW4Args* a) { return a->M > 16 && a->N * a->K >= (32 << 20); }
+// mma.sync and 25 here, N 28672 93 and 45; 4096 x 1024 stays at half the time on mma.sync). From 9 rows
+// where mma.sync reads scales often and the matrix is twice that (16 rows, K 4096, mma.sync and here:
+// groups of 32 N 8192 17.7 and 19.5, N 28672 57.5 and 37.3; of 64 N 28672 45.9 and 35.6; of 128 32.2 and
+// 34.9).
+bool w4_tc(const Dsv41GemvW4Args* a) {
+  return a->M > 16 ? a->N * a->K >= (32 << 20) : a->M > 8 && a->group % 128 && a->N * a->K >= (64 << 20);
+}
 int w4_tc_ctas(const Dsv41GemvW4Args* a) {
   return (int)std::min<int64_t>(device_sms(), cdiv64(a->N, kWtRows) * cdiv64(a->K, kWtBlock));
 }

@@ -57,10 +57,11 @@ def test_w4_matches(M, N, K, group, zeros, dt):
     (17, 8192, 4096, 128, True, BF), (48, 8200, 4128, 32, True, HF), (33, 9000, 4096, 64, False, BF),
     (32, 70000, 640, 128, True, BF), (40, 300, 129984, 96, True, HF), (48, 33000, 1056, 32, True, BF),
     (20, 5000, 8192, 512, True, BF), (9, 20000, 2048, 64, True, HF), (1, 20001, 2304, 256, False, BF),
-    (6, 9000, 4064, 32, True, BF)])
+    (6, 9000, 4064, 32, True, BF), (9, 16500, 4096, 32, False, HF), (16, 2100, 32000, 64, True, BF),
+    (13, 8200, 8256, 96, True, BF)])
 def test_w4_large(M, N, K, group, zeros, dt):
     """Matrices that fill the GPU: many row tiles a CTA, tiles that lie in several CTAs' shares, over 16
-    rows the tensor-memory kernel; the plain form in fp64 on the GPU."""
+    rows (over 8 where scales are many) the tensor-memory kernel; the plain form in fp64 on the GPU."""
     from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
     x, w, s, z = (None if t is None else t.cuda() for t in w4_case(M, N, K, group, zeros, dt, seed=3))
     w4_check(ops.gemv_w4(x, w, s, z), x, w, s, z)
