@@ -359,8 +359,8 @@ int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream);
  * j + 1, the last `window` of them with window > 0; out = sum_i softmax(scale q . k)_i v_i per
  * head, heads / kv_heads query heads a kv head, softmax and sums in fp32; sink (fp32 [heads],
  * optional) is one more score that has no value. A row that sees no key gives 0. Keys on pages out
- * of range are not seen. scale_f32: the fp32 bit pattern. Where the pages hold only short
- * sequences no scratch is needed (scratch_bytes says 0). Decode and verify rows: few rows a
+ * of range are not seen. scale_f32: the fp32 bit pattern. With short sequences or a
+ * short window no scratch may be needed (scratch_bytes says 0). Decode and verify rows: few rows a
  * sequence over a long cache. Replaces, for grouped-query heads, what back.py:189-435 of the
  * reference does for its shared latent. */
 typedef struct {

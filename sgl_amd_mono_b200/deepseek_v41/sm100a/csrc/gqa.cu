@@ -1,7 +1,9 @@
 // extern "C" entry points of the paged 8-bit cache's append and the attention over it
 // (include/dsv41_b200.h): argument checks, then the launches on the caller's stream.
+#include <algorithm>
 #include <climits>
 #include <cstring>
+#include <numeric>
 #include <type_traits>
 
 #include "../../../../include/dsv41_b200.h"
@@ -82,24 +84,30 @@ int64_t attn_go(const Dsv41PagedAttnArgs* a, F f) {
   return a->dim == 64 ? by_tiles(Int<64>()) : a->dim == 128 ? by_tiles(Int<128>()) : by_tiles(Int<256>());
 }
 
-// How the work is cut, from what the host knows: the pages that the table can name bound the steps of a
-// sequence. Short items stay whole where each can have a CTA: one launch, no scratch. Else the GPU's CTAs
-// share all steps, no more of them than there can be, and a second launch joins the pieces. Whole against
-// split, us of GPU time, dim 128: 1 row of 4 kv heads at 120 tokens 6.4 to 7.6, 380: 7.7 to 8.7, 777: 10.1
-// to 9.3; 8 rows of 8 kv heads at 777: 10.8 to 15.6; a launch less to issue besides (10.8 us a call to 15.7
-// at 777), so 8 steps (1024 tokens) where a step is cheap. With more columns or dim 256 a step costs more (4
-// rows of 4 kv heads, groups of 8, 250 tokens: 15.5 to 16.3, 500: 18.3 to 16.2; dim 256, 250: 13.0 to
-// 14.2, 500: 15.9 to 15.0): 2 steps.
+// How the work is cut, from what the host knows: the pages that the table can name and the window bound the
+// steps of an item, the rows the items. Whole items, a CTA each, take one launch and no scratch; or the
+// GPU's CTAs share all steps, no more of them than there can be, and a second launch joins the pieces.
+// Whole, the CTAs without an item idle for up to steps (1 - items / fit); split, each CTA starts and ends
+// two pieces or so. Whole against split, us of GPU time, heads of 128, groups of 8: 4 items of 3 steps 7.7
+// and 8.7, 7 steps 10.1 and 9.3 (but 10.8 and 15.7 a call); 64 items of 11 steps 13.8 and 17.6, 16 steps
+// 16.9 and 14.7; 256 of 8 steps 15.2 and 23.7; 1024 of 4 steps 45.4 and 44.3, of uneven 4 steps 36.6 and
+// 57.1. With more columns or dim 256 a step costs more: 16 items of dim 256, 3 steps 14.4 and 14.9, 4 steps
+// 15.9 and 15.0; 72 of 32 columns, 8 steps 24.2 and 23.4, 16 steps 36.3 and 29.5. At most 16 steps, since
+// one long sequence may be the only one; at most four waves of CTAs, since each has to find its item.
 struct AttnPlan {
   int64_t ctas, scratch;
   bool whole;
 };
 template <int D, int NT>
 AttnPlan attn_plan(const Dsv41PagedAttnArgs* a) {
-  const int64_t items = (a->T * (a->heads / a->kv_heads) / (8 * NT) + a->seqs) * a->kv_heads;
-  const int64_t steps = cdiv64(a->width * a->page / 16 + 1, PaShape<D, NT>::kWarps);
+  const int64_t group = a->heads / a->kv_heads, slack = 8 * NT - std::gcd<int64_t>(group, 8 * NT);
+  const int64_t items = (a->T * group + a->seqs * slack) / (8 * NT) * a->kv_heads;
+  int64_t seen = a->width * a->page;
+  if (a->window) seen = std::min(seen, a->window + a->T + 15);
+  const int64_t steps = cdiv64(cdiv64(seen, 16), PaShape<D, NT>::kWarps);
   const int64_t fit = (int64_t)device_sms() * PaShape<D, NT>::kCtas;
-  if (steps <= (PaShape<D, NT>::kO <= 32 ? 8 : 2) && items <= fit) return {std::max<int64_t>(1, items), 0, true};
+  if (steps <= 16 && items <= 4 * fit && steps * (fit - items) <= (PaShape<D, NT>::kO <= 32 ? 8 : 4) * fit)
+    return {std::max<int64_t>(1, items), 0, true};
   const int64_t ctas = std::min(fit, std::max<int64_t>(1, items * steps));
   return {ctas, ctas * (int64_t)(2 * 8 * NT * (D * sizeof(float) + sizeof(float4)) + sizeof(PaSplit)), false};
 }

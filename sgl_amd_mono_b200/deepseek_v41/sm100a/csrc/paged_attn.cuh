@@ -23,8 +23,8 @@
 // Split. The work (sequence, kv head, column tile, steps of 16 W tokens) is cut into equal
 // contiguous shares, one a CTA, whatever the lengths: each CTA finds its own from the lengths on the
 // device. A share's piece of an item that lies in several shares goes to scratch, and a second kernel
-// joins the pieces in order, so the sums do not depend on timing. Where the pages can hold only short
-// sequences and every item has a CTA, items are not split and one launch does.
+// joins the pieces in order, so the sums do not depend on timing. Where pages or window keep
+// the items short, and there are not a few items only, they are not split and one launch does.
 #pragma once
 
 #include <cfloat>
@@ -37,7 +37,7 @@ struct PagedAttnArgs {
   StepRows rows;
   KvCache cache;
   int heads, window;
-  int whole;    // items are not split: short sequences, no scratch and no second kernel
+  int whole;    // items are not split: a CTA each, no scratch and no second kernel
   float scale;  // times log2 e
   const void* q;
   void* out;

@@ -282,15 +282,18 @@ def run_attend(st, window=0, sink=False, scale=None):
     assert got is out
     ref, sizes = G.attend(q, st.k, st.v, st.kc, st.vc, st.cu, st.lens, st.table, scale, window, sk)
     used = sum(st.rows)
-    # a table with room for long sequences: the same rows, their work split and joined
+    # a table with room for long sequences, room for more rows: the same rows, their work split and joined
     wide = torch.full((len(st.rows), 4000), -1, dtype=torch.int32, device="cuda")
     wide[:, :st.table.shape[1]] = where["table"]
-    split = torch.full_like(out, 5.0)
-    kv.attend(qd, scale=scale, window=window, sink=sk_d, out=split, **{**where, "table": wide})
+    more = torch.zeros((4000,) + qd.shape[1:], dtype=qd.dtype, device="cuda")
+    split = torch.full_like(torch.cat([out, more]), 5.0)
+    kv.attend(torch.cat([qd, more]), scale=scale, window=window, sink=sk_d, out=split,
+              **{**where, "table": wide, "cu_rows": torch.arange(len(st.rows) + 1, dtype=torch.int32).cuda() if st.cu is None
+                 else where["cu_rows"]})
     for o in (out, split):
         g = o.cpu().double()
         assert bool((g[used:] == 5.0).all()), "rows behind the last sequence moved"
-        err, tol = (g - ref).abs()[:used], attn_tol(st.dt, ref, sizes)[:used]
+        err, tol = (g[:used] - ref[:used]).abs(), attn_tol(st.dt, ref, sizes)[:used]
         nan = ref[:used].isnan()
         assert torch.equal(g[:used].isnan(), nan)
         assert bool((err <= tol)[~nan].all()), (err / tol.clamp_min(1e-30))[~nan].max().item()
