@@ -139,7 +139,7 @@ extern "C" {
 int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
   if (!append_ok(a)) return DSV41_EINVAL;
   if (!a->T || !a->seqs) return DSV41_OK;
-  KvAppendArgs k = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->rope, (int)a->neox,
+  KvAppendArgs k = {step_rows(a), kv_cache(a), (int)a->heads, (int)a->rope,
                     ptr<const void>(a->q), ptr<const void>(a->k), ptr<const void>(a->v), ptr<void>(a->q_out),
                     a->q_ld, a->q_out_ld, a->k_ld, a->v_ld, ptr<const float>(a->cos_sin), a->rope_rows};
   // A warp looks through one row where most rows begin a block of their own (decode and verify rows),
@@ -150,17 +150,17 @@ int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
   const int64_t warps = cdiv64(a->T, k.window) * 2 * a->kv_heads;
   const int64_t q_threads = a->q ? a->T * cdiv64(a->heads, k.head_step) * (a->dim / 16) : 0;
   const int64_t kv_ctas = cdiv64(warps, kApThreads / 32), ctas = kv_ctas + cdiv64(q_threads, kApThreads);
-  if (ctas > INT_MAX) return DSV41_EINVAL;
+  if (ctas > UINT32_MAX / kApThreads) return DSV41_EINVAL;  // no memory holds as many rows
   k.kv_ctas = (int)kv_ctas;
   const dim3 grid((unsigned)ctas), cta(kApThreads);
-  switch (a->dim * 2 + a->f16) {
-    case 128: return launch(kv_append_kernel<false, 64>, grid, cta, 0, stream, k);
-    case 129: return launch(kv_append_kernel<true, 64>, grid, cta, 0, stream, k);
-    case 256: return launch(kv_append_kernel<false, 128>, grid, cta, 0, stream, k);
-    case 257: return launch(kv_append_kernel<true, 128>, grid, cta, 0, stream, k);
-    case 512: return launch(kv_append_kernel<false, 256>, grid, cta, 0, stream, k);
-    default: return launch(kv_append_kernel<true, 256>, grid, cta, 0, stream, k);
-  }
+  auto by_pairs = [&](auto f16, auto d) {
+    return a->neox ? launch(kv_append_kernel<f16, d, true>, grid, cta, 0, stream, k)
+                   : launch(kv_append_kernel<f16, d, false>, grid, cta, 0, stream, k);
+  };
+  auto by_dim = [&](auto f16) {
+    return a->dim == 64 ? by_pairs(f16, Int<64>()) : a->dim == 128 ? by_pairs(f16, Int<128>()) : by_pairs(f16, Int<256>());
+  };
+  return a->f16 ? by_dim(Int<1>()) : by_dim(Int<0>());
 }
 
 int64_t dsv41_paged_attn_scratch_bytes(const Dsv41PagedAttnArgs* a) {

@@ -21,7 +21,7 @@ constexpr int kApThreads = 256;
 struct KvAppendArgs {
   StepRows rows;
   KvCache cache;
-  int heads, rope, neox;
+  int heads, rope;
   const void *q, *k, *v;
   void* q_out;
   int64_t q_ld, q_out_ld, k_ld, v_ld;
@@ -36,9 +36,10 @@ struct KvAppendArgs {
 struct RopeUnit {
   int d0, d1, angle;
 };
-__device__ __forceinline__ RopeUnit rope_unit(int u, int dim, int rope, int neox) {
+template <bool NEOX>
+__device__ __forceinline__ RopeUnit rope_unit(int u, int dim, int rope) {
   const int ur = u - (dim - rope) / 16;
-  if (ur >= 0 && neox) return {dim - rope + 8 * ur, dim - rope / 2 + 8 * ur, 8 * ur};
+  if (NEOX && ur >= 0) return {dim - rope + 8 * ur, dim - rope / 2 + 8 * ur, 8 * ur};
   return {16 * u, 16 * u + 8, ur >= 0 ? 8 * ur : -1};
 }
 
@@ -69,10 +70,11 @@ __device__ __forceinline__ void rotate_pair(float& x, float& y, float c, float s
   x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
   y = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
 }
-__device__ __forceinline__ void rotate16(float (&v)[16], const Angles& a, int neox) {
+template <bool NEOX>
+__device__ __forceinline__ void rotate16(float (&v)[16], const Angles& a) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if (neox) rotate_pair(v[i], v[8 + i], a.c[i], a.s[i]);
+    if (NEOX) rotate_pair(v[i], v[8 + i], a.c[i], a.s[i]);
     else rotate_pair(v[2 * i], v[2 * i + 1], a.c[i], a.s[i]);
   }
 }
@@ -83,28 +85,28 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return lo | hi << 16;
 }
 
-// The rows [r, r + rows) of one head, tokens `pos` .. of one block, by one warp.
-template <bool F16, int D>
-__device__ __forceinline__ void append_block(const KvAppendArgs& a, int seq, int r, int rows, int64_t pos, int item) {
+// The rows [r, r + rows) of one head, tokens `pos` .. of one block (its `in`th token on), by one warp.
+template <bool F16, int D, bool NEOX>
+__device__ __forceinline__ void append_block(const KvAppendArgs& a, int seq, int r, int rows, int pos, int in, int item) {
   using T = typename Act<F16>::T;
   constexpr int UNITS = D / 16, PER = 32 / UNITS;  // lanes a row, rows at a time
   const int lane = threadIdx.x & 31, kvh = a.cache.kv_heads, block = a.cache.block, page = a.cache.page;
-  const int pg = token_page(a.rows, a.cache, seq, (int)pos);
+  const int pg = token_page(a.rows, a.cache, seq, pos);
   if (pg < 0) return;
   const bool is_k = item < kvh;
   const int hk = is_k ? item : item - kvh;
-  const int in = (int)(pos % block), off = (int)(pos % page) - in;  // the block's first token in its page
+  const int off = pos % page - in;  // the block's first token in its page
   const T* x = reinterpret_cast<const T*>(is_k ? a.k : a.v) + hk * D;
   const int64_t ld = is_k ? a.k_ld : a.v_ld;
   const int64_t head = (int64_t)pg * kvh + hk;
   uint8_t* dst = (is_k ? a.cache.k : a.cache.v) + (head * page + off) * D;
   uint8_t* cp = (is_k ? a.cache.k_codes : a.cache.v_codes) + head * (page / block) + off / block;
   const int rope = is_k ? a.rope : 0;
-  const RopeUnit ru = rope_unit(lane % UNITS, D, rope, a.neox);
+  const RopeUnit ru = rope_unit<NEOX>(lane % UNITS, D, rope);
   const int old = in ? *cp : 0;
-  // the lane's units of rows i, i + PER, ..: KEEP of them stay in registers for the second pass (4 keep all
-  // of a block of 16 rows of 128 dims, but with 2 four CTAs fit an SM: ragged prompts 53 us against 59)
-  constexpr int KEEP = 2;
+  // the lane's units of rows i, i + PER, ..: the first KEEP stay in registers for the second pass, the others
+  // come from L1 again (ragged prompts: 1 47.4 us, 2 48.9, 4 over 59 at the two CTAs an SM that it leaves)
+  constexpr int KEEP = 1;
   auto load = [&](int i, uint4 (&w)[2]) {
     const T* row = x + (r + i) * ld;
     w[0] = ldg16(row + ru.d0);
@@ -116,7 +118,7 @@ __device__ __forceinline__ void append_block(const KvAppendArgs& a, int seq, int
     if (rope && ru.angle >= 0) {
       Angles an;
       load_angles(a.cos_sin + rope_row(pos + i, a.rope_rows) * rope, rope, ru.angle, an);
-      rotate16(v, an, a.neox);
+      rotate16<NEOX>(v, an);
     }
   };
   const int i0 = lane / UNITS;
@@ -191,7 +193,7 @@ __device__ __forceinline__ int row_seq_search(const StepRows& s, int r) {
 
 // CTAs [0, kv_ctas): a warp a (window of rows, key or value head); the others: a thread a (row, head_step
 // query heads, unit).
-template <bool F16, int D>
+template <bool F16, int D, bool NEOX>
 __global__ void __launch_bounds__(kApThreads, 4) kv_append_kernel(const KvAppendArgs a) {
   using T = typename Act<F16>::T;
   constexpr int UNITS = D / 16;
@@ -199,10 +201,10 @@ __global__ void __launch_bounds__(kApThreads, 4) kv_append_kernel(const KvAppend
   const StepRows& st = a.rows;
   if ((int)blockIdx.x < a.kv_ctas) {
     const int lane = threadIdx.x & 31, items = 2 * a.cache.kv_heads, block = a.cache.block;
-    const int64_t wi = (int64_t)blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5);
-    const int64_t w0 = wi / items * a.window;
+    const uint32_t wi = blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5), window = wi / items;
+    const int64_t w0 = (int64_t)window * a.window;
     if (w0 >= st.T) return;
-    const int item = (int)(wi % items), w1 = (int)min(w0 + a.window, (int64_t)st.T);
+    const int item = wi - window * items, w1 = (int)min(w0 + a.window, (int64_t)st.T);
     const int64_t cap = (int64_t)st.width * a.cache.page;
     int r = (int)w0, seq = row_seq(st, r, lane);
     while (r < w1 && seq >= 0 && seq < st.seqs) {
@@ -216,31 +218,24 @@ __global__ void __launch_bounds__(kApThreads, 4) kv_append_kernel(const KvAppend
       if (pos < 0) {
         rows = (int)min((int64_t)rows, -pos);
       } else {
-        rows = min(min(rows, block - (int)(pos % block)), st.T - r);
+        const int in = (uint32_t)pos % block;  // pos < lens[seq]
+        rows = min(min(rows, block - in), st.T - r);
         // the block's first new row leads: the sequence's first, one at the block's start, or token 0
-        if ((r == first || pos % block == 0) && pos < cap) append_block<F16, D>(a, seq, r, rows, pos, item);
+        if ((r == first || !in) && pos < cap) append_block<F16, D, NEOX>(a, seq, r, rows, (int)pos, in, item);
       }
       r += rows;
     }
     return;
   }
   const int groups = (a.heads + a.head_step - 1) / a.head_step;
-  const int64_t ti = (int64_t)(blockIdx.x - a.kv_ctas) * kApThreads + threadIdx.x;
-  const int64_t row = ti / (groups * UNITS);
+  const uint32_t ti = (blockIdx.x - a.kv_ctas) * kApThreads + threadIdx.x, per = groups * UNITS;
+  const int64_t row = ti / per;
   if (row >= st.T) return;
-  const int r = (int)row, u = (int)(ti % UNITS), h0 = (int)(ti / UNITS % groups) * a.head_step;
-  const int seq = row_seq_search(st, r);
-  if (seq < 0) return;
-  const RopeUnit ru = rope_unit(u, D, a.rope, a.neox);
-  Angles an;
-  if (a.rope && ru.angle >= 0) {
-    const int64_t pos = (int64_t)st.lens[seq] - (st.cu_rows ? st.cu_rows[seq + 1] : seq + 1) + r;
-    load_angles(a.cos_sin + rope_row(max(pos, (int64_t)0), a.rope_rows) * a.rope, a.rope, ru.angle, an);
-  }
+  const int r = (int)row, u = ti % UNITS, h0 = (ti - (uint32_t)r * per) / UNITS * a.head_step;
+  const RopeUnit ru = rope_unit<NEOX>(u, D, a.rope);
   const T* x = reinterpret_cast<const T*>(a.q) + row * a.q_ld;
-  T* y = reinterpret_cast<T*>(a.q_out) + row * a.q_out_ld;
-  // every load ahead of the first store (plain loads: the queries may be rotated in place, a thread's own
-  // values each)
+  // Every load ahead of the first store and of the search for the sequence (plain loads: the queries may be
+  // rotated in place, a thread's own values each).
   constexpr int HEADS = 4;
   uint4 in[HEADS][2];
 #pragma unroll
@@ -249,13 +244,21 @@ __global__ void __launch_bounds__(kApThreads, 4) kv_append_kernel(const KvAppend
       in[n][0] = *reinterpret_cast<const uint4*>(x + (h0 + n) * D + ru.d0);
       in[n][1] = *reinterpret_cast<const uint4*>(x + (h0 + n) * D + ru.d1);
     }
+  const int seq = row_seq_search(st, r);
+  if (seq < 0) return;
+  Angles an;
+  if (a.rope && ru.angle >= 0) {
+    const int64_t pos = (int64_t)st.lens[seq] - (st.cu_rows ? st.cu_rows[seq + 1] : seq + 1) + r;
+    load_angles(a.cos_sin + rope_row(max(pos, (int64_t)0), a.rope_rows) * a.rope, a.rope, ru.angle, an);
+  }
+  T* y = reinterpret_cast<T*>(a.q_out) + row * a.q_out_ld;
 #pragma unroll
   for (int n = 0; n < HEADS; ++n)
     if (n < a.head_step && h0 + n < a.heads) {
       float v[16];
       unpack8<F16>(in[n][0], v);
       unpack8<F16>(in[n][1], v + 8);
-      if (a.rope && ru.angle >= 0) rotate16(v, an, a.neox);
+      if (a.rope && ru.angle >= 0) rotate16<NEOX>(v, an);
       uint32_t w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = Act<F16>::pack(v[2 * e], v[2 * e + 1]);
