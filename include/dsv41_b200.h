@@ -313,8 +313,8 @@ int dsv41_argmax_decode(const Dsv41ArgmaxArgs* a, void* stream);
  * [N, K / group] (values 0 .. 15) or 0 for 8 everywhere; x [M, x_ld] and y [M, y_ld] bf16 (below
  * 2^63 in magnitude), or f16 with f16 = 1. M <= 48, K a multiple of group, group a multiple of 32;
  * w and x 16-byte aligned, x_ld a multiple of 8. An infinity or NaN in a row of x makes that row of
- * y not finite, one in a scale that column. Up to 8 rows need no scratch. No counterpart in the
- * reference (its dense projections are FP8). */
+ * y not finite, one in a scale that column. Up to 8 rows, and N K below 2^25, need no
+ * scratch. No counterpart in the reference (its dense projections are FP8). */
 typedef struct {
   int64_t w, scales, zeros, x, y;     /* device pointers */
   int64_t M, N, K, group, x_ld, y_ld, f16;

@@ -7,7 +7,8 @@
 // the subnormal n 2^-24 of f16 (n 2^-133 of bf16), exact like every product of m16n8k16 with x (bf16 x
 // is staged times 2^64, so that products stay in fp32's normal range). Zero points come off the fp32
 // sums: sum x (n - z) = sum x n - z sum x, the last sum taken once with the rows of x in shared memory
-// (where they do not fit, by the same instruction from a fragment of ones); it costs the sums an error of at most 16 / |n - z| of their own.
+// (where they do not fit, by the same instruction from a fragment of ones); it costs the sums an error of
+// at most 16 / |n - z| of their own.
 // Weight rows are the mma's M, the rows of x its N. One word of a lane holds 8 consecutive k of a row;
 // masking word >> 4 i gives the pair (k_i, k_(i + 4)), and x is paired up the same way, so no nibble is
 // moved for order's sake: 7 logic instructions for 8 weights.
@@ -15,6 +16,9 @@
 // A CTA takes 16 R weight rows at a time, its warps chunks of 256 k (128 bytes a row) in turn; every
 // warp streams its chunks through a ring of its own by 16-byte cp.async, across row tiles without a
 // pause. The warps' sums meet in shared memory in warp order, so the result does not depend on timing.
+//
+// One row: 1024 x 1024 2.3 us (launch and one latency), 8192 x 4096 6.6 us (2.7 TB/s: two tiles a CTA),
+// 65536 x 8192 at 4.3 TB/s, where the logic pipe issues 63 % of what it can and DRAM is at 53 %.
 #pragma once
 
 #include <type_traits>
@@ -47,9 +51,9 @@ struct W4Shape {
   static constexpr int kEntries = 8 / GS;                     // scales a row of a chunk
   // weights; without a table of the tile's scales {-zero, scale} of each entry and row
   static constexpr int kStage = kRows * (128 + (ST ? 0 : 8 * kEntries));
-    // two or three CTAs an SM beat a deeper ring (N 129280, K 4096, one row: 69 us with 2 stages of 32
+  // two or three CTAs an SM beat a deeper ring (N 129280, K 4096, one row: 69 us with 2 stages of 32
   // rows, 92 us with 3 stages and so one CTA)
-    static constexpr int kStages = 2;
+  static constexpr int kStages = 2;
   static constexpr int kRing = kW4Warps * kStages * kStage;
   // one tile's partial sums, two of them behind the ring; then the rows of x, where they fit
   static __host__ __device__ constexpr int sums(int M) { return kW4Warps * kRows * M * 4; }
@@ -141,7 +145,8 @@ __global__ void __launch_bounds__(32 * kW4Warps) gemv_w4_kernel(const GemvW4Args
       for (int o = tid * 16; o < zb; o += sharers * 16) cp_async16_part(dst + sb + o, zp, o, rows * groups);
   };
 
-  // Without it a chunk's scales and zeros go through registers: loaded when the chunk is issued, stored (in fp32) when the next one is, so that nothing waits for them.
+  // Without it a chunk's scales and zeros go through registers: loaded when the chunk is issued, stored (in
+  // fp32) when the next one is, so that nothing waits for them.
   uint32_t sc[R][EL], ze[R][EL];
   // the next chunk to issue: its number, its place in the warp's chunks of a tile, the tile
   int is_j = 0, is_c = 0, is_tile = blockIdx.x, is_st = 0, is_it = 0;

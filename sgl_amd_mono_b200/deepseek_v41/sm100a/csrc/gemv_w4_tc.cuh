@@ -13,6 +13,10 @@
 // issue of the two accumulators, 2 .. 5 x, 8 .. 15 converters. The blocks of all row tiles are cut into equal
 // contiguous shares, one a CTA; tiles that lie in several shares are joined from scratch in order by
 // a second kernel.
+//
+// 48 rows of 129280 x 4096, groups of 64: 142 us, 2.1 TB/s of the weights and scales that bound it in
+// principle (46 us). The hand-over bounds it now: two converter warps a scheduler each convert, wait for the
+// MMA and read back in turn (logic pipe 44 %, tensor pipe 18 %, DRAM 26 %). Roundings: none but y's.
 #pragma once
 
 #include "gemv_w4.cuh"

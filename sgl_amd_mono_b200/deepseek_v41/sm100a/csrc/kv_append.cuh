@@ -10,6 +10,10 @@
 // pieces that hold 8 whole rotation pairs and share 8 angles, side by side for pairs (2j, 2j + 1) and
 // half a rotation apart for (j, j + rope / 2). A block's rows are looked at twice, for the largest
 // magnitude and to be written, some of them in registers and the others from L1.
+//
+// One token 3.2 us and 8 sequences of 6 rows 3.6: dependent latencies (row, length, page, code). Prompts of
+// 10266 rows, 32 query and 8 kv heads of 128: 47 us (5.0 TB/s of 236 MB). The queries alone take 29 us, a copy of
+// them 27; the keys and values 23, which is latency and the second look, not bytes (10 us).
 #pragma once
 
 #include "gqa.cuh"

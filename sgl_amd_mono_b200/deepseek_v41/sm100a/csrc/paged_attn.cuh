@@ -25,6 +25,11 @@
 // device. A share's piece of an item that lies in several shares goes to scratch, and a second kernel
 // joins the pieces in order, so the sums do not depend on timing. Where pages or window keep
 // the items short, and there are not a few items only, they are not split and one launch does.
+//
+// 4 rows of 64 heads over 131072 tokens, 8 kv heads: 182 us, 0.90 of the time its bytes take. With up to 16
+// columns DRAM bounds it; with more, latencies between the dependent products and conversions of a tile
+// on the two or three warps a scheduler that their registers leave (8 x 6 rows, 24 columns, at 32768
+// tokens: 147 us for 82 us of bytes; tensor pipe 30 %, 1.4 instructions a cycle of 4).
 #pragma once
 
 #include <cfloat>

@@ -77,9 +77,10 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch
                                f"want [{M}, {N}] {dtype} on {x.device}, contiguous rows")
         a.y_ld = y_ld
     a.y = out.data_ptr()
-    if M > 8:  # fewer rows need no scratch
+    if M > 8 and N * K >= 1 << 25:  # fewer rows and smaller matrices need no scratch
         need = ext.query("dsv41_gemv_w4_scratch_bytes", a)
-        scratch = w.new_empty((need,))
-        a.scratch, a.scratch_bytes = scratch.data_ptr(), need
+        if need:
+            scratch = w.new_empty((need,))
+            a.scratch, a.scratch_bytes = scratch.data_ptr(), need
     ext.call("dsv41_gemv_w4", a, stream)
     return out

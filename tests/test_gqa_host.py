@@ -79,6 +79,8 @@ def test_scratch_that_does_not_do_is_refused(short):
     assert ext.query("dsv41_paged_attn_scratch_bytes", abi.PagedAttnArgs(**long)) > 0
     assert _call("dsv41_paged_attn", abi.PagedAttnArgs(**{**long, **short})) == -3
     assert ext.query("dsv41_gemv_w4_scratch_bytes", abi.GemvW4Args(**{**W4, "M": 8})) == 0
+    small = {**W4, "M": 48, "N": 8191, "K": 4096, "x_ld": 4096, "y_ld": 8192}
+    assert ext.query("dsv41_gemv_w4_scratch_bytes", abi.GemvW4Args(**small)) == 0
     big = {**W4, "M": 48, "N": 8192, "K": 4096, "x_ld": 4096, "y_ld": 8192}
     assert ext.query("dsv41_gemv_w4_scratch_bytes", abi.GemvW4Args(**big)) > 0
     assert _call("dsv41_gemv_w4", abi.GemvW4Args(**{**big, **short})) == -3
