@@ -81,7 +81,8 @@ def test_w4_unaligned_scales_and_tiny_scales():
         w4_check(ops.gemv_w4(x, w, st, z), x, w, st, z)
 
 
-@pytest.mark.parametrize("M,N,K,group", [(3, 40, 1024, 128), (48, 1000, 2304, 32), (7, 19, 160, 32)])
+@pytest.mark.parametrize("M,N,K,group", [(3, 40, 1024, 128), (48, 1000, 2304, 32), (7, 19, 160, 32), (11, 2100, 32000, 64),
+                                         (20, 9000, 4096, 64)])
 def test_w4_strides_and_neighbours(M, N, K, group):
     """Rows of x further apart than K, an output inside a wider buffer whose other values stay."""
     from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
