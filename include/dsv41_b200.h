@@ -360,7 +360,8 @@ int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream);
  * head, heads / kv_heads query heads a kv head, softmax and sums in fp32; sink (fp32 [heads],
  * optional) is one more score that has no value. A row that sees no key gives 0. Keys on pages out
  * of range are not seen. scale_f32: the fp32 bit pattern. With short sequences or a
- * short window no scratch may be needed (scratch_bytes says 0). Decode and verify rows: few rows a
+ * short window no scratch may be needed (scratch_bytes says 0); what a call needs follows from its own
+ * sizes, and fewer rows may need more. Decode and verify rows: few rows a
  * sequence over a long cache. Replaces, for grouped-query heads, what back.py:189-435 of the
  * reference does for its shared latent. */
 typedef struct {
