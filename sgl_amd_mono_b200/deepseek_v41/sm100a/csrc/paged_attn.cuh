@@ -16,9 +16,12 @@
 // wastes little, and O^T = V^T P^T takes P from S's registers by a transposing movmatrix.
 //
 // Roundings. K and V become f16 exactly; q is scaled per column by a power of two into f16's range
-// (exact but for values 2^-29 below the column's largest). Scores, weights, sums and O are fp32; only
-// the weights are rounded to f16 for the second product: half a step of 2^-11 of each weight, and
-// those below 2^-21 of the largest keep an absolute 2^-32 of it.
+// (exact but for values 2^-29 below the column's largest). Scores, weights, sums and O are fp32. A
+// weight enters the second product as two f16 numbers, its head and what the head leaves, which
+// keeps it to 2^-22 of itself and 2^-32 of the column's largest. The head alone (2^-11) showed: outputs
+// 8e-4 (bf16) and 3e-4 (f16) of their size away from those of fp32 weights, now 1e-4 or less but over
+// the longest contexts. The tails' product costs 2 % with one column tile (95 to 97 us for 48 rows at
+// 8192 tokens, 182 to 187 for 4 at 131072) and 13 % with three (147 to 167).
 //
 // Split. The work (sequence, kv head, column tile, steps of 16 W tokens) is cut into equal
 // contiguous shares, one a CTA, whatever the lengths: each CTA finds its own from the lengths on the
@@ -26,10 +29,11 @@
 // joins the pieces in order, so the sums do not depend on timing. Where pages or window keep
 // the items short, and there are not a few items only, they are not split and one launch does.
 //
-// 4 rows of 64 heads over 131072 tokens, 8 kv heads: 182 us, 0.90 of the time its bytes take. With up to 16
+// 4 rows of 64 heads over 131072 tokens, 8 kv heads: 187 us, its bytes take 0.88 of that. With up to 16
 // columns DRAM bounds it; with more, latencies between the dependent products and conversions of a tile
 // on the two or three warps a scheduler that their registers leave (8 x 6 rows, 24 columns, at 32768
-// tokens: 147 us for 82 us of bytes; tensor pipe 30 %, 1.4 instructions a cycle of 4).
+// tokens: 167 us for 82 us of bytes), some of which spill (24 columns of 128 dims: 255 registers, 232
+// bytes reloaded in bf16 and 208 in f16).
 #pragma once
 
 #include <cfloat>
@@ -488,15 +492,21 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
             for (int i = 0; i < KS; ++i) o[n][i][e] *= f, o[n][i][e + 2] *= f;
           }
       }
-      uint32_t pb[NT][2];
+      uint32_t ph[NT][2], pl[NT][2];  // the weights' f16 heads, and what those leave
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) l[n][e] += ex2(s[n][e] - top[n][e]) + ex2(s[n][e + 2] - top[n][e]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] = ex2(s[n][e] + (ev + 7.f - ref[n][e & 1]));
-        pb[n][0] = movmatrix(pa_pack(s[n][0], s[n][1]));
-        pb[n][1] = movmatrix(pa_pack(s[n][2], s[n][3]));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = s[n][2 * e], y = s[n][2 * e + 1];
+          const uint32_t head = pa_pack(x, y);
+          const float2 h = Act<true>::unpack(head);
+          ph[n][e] = movmatrix(head);
+          pl[n][e] = movmatrix(pa_pack(x - h.x, y - h.y));
+        }
       }
 
       // O^T += V^T P^T: lane (g, t) reads tokens t, 7 - t, t + 8, 15 - t (kappa of the mma's k = 2t,
@@ -543,7 +553,9 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
           e4m3x4_f16(__byte_perm(v[0][i], v[1][i], sel), a0, a1);
           e4m3x4_f16(__byte_perm(v[2][i], v[3][i], sel), a2, a3);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) pa_mma(o[n][2 * i + h], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+          for (int n = 0; n < NT; ++n) pa_mma(o[n][2 * i + h], a0, a1, a2, a3, ph[n][0], ph[n][1]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) pa_mma(o[n][2 * i + h], a0, a1, a2, a3, pl[n][0], pl[n][1]);
         }
       if (edge && __any_sync(0xffffffffu, nan)) {
         // this lane's dims of each token again: what holds NaN makes NaN of the columns that see it

@@ -1,0 +1,58 @@
+"""The grouped-query operators where their first tests do not reach: instances of the kernels that
+other sizes choose, the ends of the accepted ranges, the precision of the attention's weights."""
+
+import copy
+import math
+
+import pytest
+import torch
+
+from oracle import gqa as G
+from test_gqa_gpu import BF, HF, Step, attn_tol, half_step, rope_table, run_append, run_attend, same_bytes, w4_case, w4_check
+
+pytestmark = pytest.mark.gpu
+
+
+def attend_both(st, scale, window=0, sink=None, rows_out=None):
+    """The attention with the step's own table and with one so wide that the work is split and joined;
+    the rows and with them the kernel's instance stay."""
+    kv, where = st.cache(), st.where()
+    q = st.split(st.qkv.cuda())[0]
+    wide = torch.full((len(st.rows), 4000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :st.table.shape[1]] = where["table"]
+    sink = None if sink is None else sink.cuda()
+    return [kv.attend(q, scale=scale, window=window, sink=sink, **{**where, "table": t}).cpu()
+            for t in (where["table"], wide)]
+
+
+# (dim, query heads a kv head): with one row a sequence 8, 16, 24 and 32 columns together
+INSTANCES = [(64, 4), (64, 12), (64, 20), (64, 32), (128, 8), (128, 12), (128, 20), (128, 32), (256, 5), (256, 16)]
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("dim,group", INSTANCES)
+def test_attend_weights_keep_fp32(dim, group, dt):
+    """The weights enter the second product with fp32's precision. Queries of one dim that is not zero
+    make every score a single product, so nothing else is off by more than this bound:
+
+    * an exponent: the score's rounding (1.5 steps of 2^-24 of at most 8), two additions of the
+      references and scales (2^-24 of at most 32 each), as much once more for the sum, ex2's 2^-22
+      where a weight, a term of the sum or a factor between references is made: 2^-17 in all
+    * a weight: head and tail in f16 leave 2^-22 of it, and 2^-32 of the largest where the tail ends
+    * fp32 sums: at most 3 tiles a warp, 17 additions for each product of head and of tail, then the
+      joins of 12 warps and 4 pieces: 120 additions, each off by a step (2^-23) of sum p |v| at most
+    * the factor and its quotient: 2^-22 of the value; and the output's rounding
+    """
+    st = Step([1, 1, 1, 1], [300, 40, 17, 0], 2 * group, 2, dim, 32, 16, dt, seed=31)
+    q = st.split(st.qkv)[0]
+    keep = q[..., 5].clone()
+    q.zero_()
+    q[..., 5] = keep
+    ref, (vabs, sabs, top, seen) = G.attend(q, st.k, st.v, st.kc, st.vc, st.cu, st.lens, st.table, 1 / 16)
+    assert sabs.max().item() * 1.4427 < 8
+    tol = (half_step(dt) + 2.0 ** -22) * ref.abs() + (2.0 ** -17 + 2.0 ** -22 + 120 * 2.0 ** -23) * vabs \
+        + (seen * 2.0 ** -32 * 448 * top)[..., None]
+    tol = tol + 2.0 ** -25 if dt == HF else tol
+    for o in attend_both(st, 1 / 16):
+        off = ((o.double() - ref).abs() / tol.clamp_min(1e-30)).max().item()
+        assert off <= 1, off
