@@ -8,7 +8,9 @@ pages ``table[s]``; its rows are its last tokens. The rows ``[T, heads, dim]`` o
 one after the other: ``cu_rows[s] .. cu_rows[s + 1]`` are sequence ``s``'s, or row ``s`` alone with
 ``cu_rows=None``. Everything a call needs stays on the device, so a call can be captured in a CUDA
 graph with its lengths and pages changed between replays; a padded batch gives its unused
-sequences no rows (or length 0). Host-side argument errors raise ``RuntimeError``.
+sequences no rows (or length 0). A ``PagedKV`` stays with the tensors that it was made of: they
+cannot be replaced, a copy has tensors of its own, and calls are refused once one of them has moved
+to other memory. Host-side argument errors raise ``RuntimeError``.
 """
 
 from __future__ import annotations
@@ -48,11 +50,12 @@ class PagedKV:
             if t.shape != tuple(shape) or t.element_size() != 1 or not t.is_contiguous() or t.device != k.device:
                 raise RuntimeError(f"PagedKV: {name} {tuple(t.shape)} {t.dtype} on {t.device}: want contiguous bytes "
                                    f"{tuple(shape)} on {k.device}")
-        self.k, self.v, self.k_codes, self.v_codes = k, v, k_codes, v_codes
+        self._tensors = (k, v, k_codes, v_codes)
+        self._at = (k.data_ptr(), v.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr())
         self.pages, self.kv_heads, self.page, self.dim, self.block = pages, heads, page, dim, page // per
         self._dev = k.get_device()
-        cache = dict(kv_heads=heads, dim=dim, k_cache=k.data_ptr(), v_cache=v.data_ptr(), k_codes=k_codes.data_ptr(),
-                     v_codes=v_codes.data_ptr(), pages=pages, page=page, block=self.block)
+        cache = dict(zip(("k_cache", "v_cache", "k_codes", "v_codes"), self._at), kv_heads=heads, dim=dim, pages=pages,
+                     page=page, block=self.block)
         self._append_args, self._attend_args = bytes(abi.KvAppendArgs(**cache)), bytes(abi.PagedAttnArgs(**cache))
 
     @classmethod
@@ -64,6 +67,16 @@ class PagedKV:
         data, codes = (pages, kv_heads, page, dim), (pages, kv_heads, page // block)
         return cls(torch.zeros(data, **u8), torch.zeros(data, **u8), torch.zeros(codes, **u8),
                    torch.zeros(codes, **u8))
+
+    # The calls' argument blocks hold the tensors' addresses, so the tensors are read-only attributes and
+    # a copy (deepcopy, pickle) is made from its own.
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_codes = property(lambda self: self._tensors[2])
+    v_codes = property(lambda self: self._tensors[3])
+
+    def __reduce__(self):
+        return type(self), self._tensors
 
     # ------------------------------------------------------------ checks
     def _rows(self, x: torch.Tensor, name: str, rows: int, dtype: torch.dtype, heads: int) -> tuple[int, int]:
@@ -84,6 +97,9 @@ class PagedKV:
               cu_rows: torch.Tensor | None) -> tuple[int, torch.dtype]:
         """Check the step's tensors and fill in what the two calls share: (rows, their type)."""
         dev, i32, dtype = self._dev, torch.int32, x.dtype
+        kt, vt, kc, vc = self._tensors
+        if (kt.data_ptr(), vt.data_ptr(), kc.data_ptr(), vc.data_ptr()) != self._at:
+            raise RuntimeError(f"{name}: a cache tensor has moved since the PagedKV was made of it; make another")
         if x.dim() != 3:
             raise RuntimeError(f"{name}: {tuple(x.shape)}: want [rows, heads, {self.dim}]")
         if dtype is not torch.bfloat16 and dtype is not torch.float16:

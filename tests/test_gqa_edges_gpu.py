@@ -56,3 +56,20 @@ def test_attend_weights_keep_fp32(dim, group, dt):
     for o in attend_both(st, 1 / 16):
         off = ((o.double() - ref).abs() / tol.clamp_min(1e-30)).max().item()
         assert off <= 1, off
+
+
+def test_a_snapshot_of_the_cache_is_its_own():
+    """What is appended to a deep copy leaves the cache that it was taken of as it was."""
+    st = Step([3, 1], [40, 20], 4, 2, 64, 16, 16, BF, seed=32)
+    kv = st.cache()
+    snap = copy.deepcopy(kv)
+    q, k, v = st.split(st.qkv.cuda())
+    w = st.where()
+    before = kv.attend(q, scale=0.125, **w)
+    snap.append(k, v, **w)
+    for a, b in ((kv.k, st.k), (kv.v, st.v), (kv.k_codes, st.kc), (kv.v_codes, st.vc)):
+        assert torch.equal(a.cpu(), b)
+    assert torch.equal(kv.attend(q, scale=0.125, **w), before)
+    kv.append(k, v, **w)
+    assert torch.equal(kv.k, snap.k) and torch.equal(kv.v_codes, snap.v_codes)
+    assert torch.equal(kv.attend(q, scale=0.125, **w), snap.attend(q, scale=0.125, **w))

@@ -164,3 +164,42 @@ def test_plain_attention_masks():
     sunk, _ = G.attend(q, k, v, codes, codes, None, [0, 9], table, 0.1, window=1, sink=torch.tensor([0.5, 0.5]))
     share = 1 / (1 + math.exp(0.5 - z[0].item()))
     assert torch.allclose(sunk[1, 0], out[1, 0] * share, rtol=1e-12)
+
+
+def test_a_cache_stays_with_its_tensors():
+    """Copies address their own tensors; tensors cannot be replaced, and a moved one is refused."""
+    import copy
+    import io
+
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import abi
+    from sgl_amd_mono_b200.deepseek_v41.sm100a.paged import PagedKV
+
+    def addresses(kv):
+        both = [t.from_buffer_copy(b) for t, b in ((abi.KvAppendArgs, kv._append_args), (abi.PagedAttnArgs, kv._attend_args))]
+        return [[getattr(a, n) for n in ("k_cache", "v_cache", "k_codes", "v_codes")] for a in both]
+
+    def own(kv):
+        return [[t.data_ptr() for t in (kv.k, kv.v, kv.k_codes, kv.v_codes)]] * 2
+
+    kv = PagedKV.empty(4, 32, 2, 64, device="cpu")
+    kv.k[1, 0, 2, 3] = 7
+    buf = io.BytesIO()
+    torch.save(kv, buf)
+    deep, shallow, saved = copy.deepcopy(kv), copy.copy(kv), torch.load(io.BytesIO(buf.getvalue()), weights_only=False)
+    for c in (kv, deep, shallow, saved):
+        assert addresses(c) == own(c) and (c.pages, c.page, c.block, c.kv_heads, c.dim) == (4, 32, 16, 2, 64)
+        assert int(c.k[1, 0, 2, 3]) == 7
+    assert shallow.k is kv.k and len({c.k.data_ptr() for c in (kv, deep, saved)}) == 3
+    for name in ("k", "v", "k_codes", "v_codes"):
+        with pytest.raises(AttributeError):
+            setattr(kv, name, getattr(deep, name))
+    x = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    where = dict(lens=torch.ones(1, dtype=torch.int32), table=torch.zeros(1, 1, dtype=torch.int32))
+    args = abi.KvAppendArgs()
+    kv._step(args, x, "k", where["lens"], where["table"], None)
+    assert args.T == 1
+    for name, t in (("k", kv.k), ("v_codes", kv.v_codes)):
+        moved = copy.deepcopy(kv)
+        getattr(moved, name).set_(t.clone())
+        with pytest.raises(RuntimeError, match="moved"):
+            moved._step(abi.KvAppendArgs(), x, "k", where["lens"], where["table"], None)
