@@ -65,9 +65,13 @@ struct PaSplit {
 
 // One sequence's work: its rows, its tiles [tile0, tile0 + tiles) and what that makes in units.
 struct SeqWork {
-  int row0, n, cols, cts, tile0, tiles, steps, end;  // end: tokens its last row sees (unclamped)
+  int row0, n, cols, cts, tile0, tiles, steps, end;  // end: tokens its last row sees, up to 2^31 - 1
   long long units;
 };
+
+// The first token that a row sees which sees the tokens before vis. (A row before the sequence's first
+// token has vis <= 0, and a window may be 2^31 - 1, so their difference need not fit 32 bits.)
+__device__ __forceinline__ int window_low(int vis, int window) { return window && vis > window ? vis - window : 0; }
 
 template <int NT, int W>
 __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
@@ -75,13 +79,12 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
   w.row0 = a.rows.cu_rows ? a.rows.cu_rows[s] : s;
   w.n = a.rows.cu_rows ? a.rows.cu_rows[s + 1] - w.row0 : 1;
   w.n = w.row0 < 0 || w.row0 > a.rows.T ? 0 : max(0, min(w.n, a.rows.T - w.row0));
-  w.end = a.rows.lens[s];
+  w.end = max(a.rows.lens[s], 0);
   const int kvh = a.cache.kv_heads;
   w.cols = w.n * (a.heads / kvh);
   w.cts = (w.cols + 8 * NT - 1) / (8 * NT);
-  const int hi = min(max(w.end, 0), a.rows.width * a.cache.page);
-  const int lo = a.window ? max(0, w.end - w.n + 1 - a.window) : 0;
-  w.tile0 = lo / 16;
+  const int hi = min(w.end, a.rows.width * a.cache.page);
+  w.tile0 = window_low(w.end - w.n + 1, a.window) / 16;
   w.tiles = max(0, (hi + 15) / 16 - w.tile0);
   w.steps = max(1, (w.tiles + W - 1) / W);
   w.units = (long long)w.cts * kvh * (a.whole ? 1 : w.steps);
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
     const int cap = a.rows.width * page;
     const int vis0 = w.end - w.n + 1;
     auto vis = [&](int j) { return vis0 + j; };
-    auto low = [&](int j) { return a.window ? max(0, vis(j) - a.window) : 0; };
+    auto low = [&](int j) { return window_low(vis(j), a.window); };
     const int any_lo = low(j0), any_hi = min(vis(j1), cap), all_lo = low(j1), all_hi = min(vis(j0), cap);
 
     // Q: column n's dims 64 c + 16 t + 4 q + {0 .. 3} are step 4 c + q's fragment of lane (n, t)

@@ -73,3 +73,24 @@ def test_a_snapshot_of_the_cache_is_its_own():
     kv.append(k, v, **w)
     assert torch.equal(kv.k, snap.k) and torch.equal(kv.v_codes, snap.v_codes)
     assert torch.equal(kv.attend(q, scale=0.125, **w), snap.attend(q, scale=0.125, **w))
+
+
+@pytest.mark.parametrize("window", [1 << 30, (1 << 31) - 8, (1 << 31) - 1])
+@pytest.mark.parametrize("rows,lens", [([6, 2], [3, 2]), ([6, 1], [0, 1]), ([9, 3], [8, 50])])
+def test_attend_windows_up_to_the_last(window, rows, lens):
+    """A window that no sequence fills is none, with more rows than tokens too."""
+    st = Step(rows, lens, 4, 2, 64, 16, 16, BF, seed=33)
+    a, b = attend_both(st, 0.125)
+    c, d = attend_both(st, 0.125, window=window)
+    assert torch.equal(a, c) and torch.equal(b, d)
+    ref, sizes = G.attend(st.split(st.qkv)[0], st.k, st.v, st.kc, st.vc, st.cu, st.lens, st.table, 0.125, window)
+    assert bool(((c.double() - ref).abs() <= attn_tol(BF, ref, sizes)).all()) and bool(c.any())
+
+
+def test_attend_negative_lengths_see_nothing():
+    """A length below zero holds no token, whatever its size."""
+    st = Step([2, 1, 3], [0, 20, 0], 4, 2, 64, 16, 16, BF, seed=34)
+    st.lens[0], st.lens[2] = -5, -(1 << 31)
+    for window in (0, 7, (1 << 31) - 1):
+        for o in attend_both(st, 0.125, window=window):
+            assert not bool(o[:2].any()) and not bool(o[3:].any()) and bool(o[2].any())
