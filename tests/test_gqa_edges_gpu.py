@@ -94,3 +94,16 @@ def test_attend_negative_lengths_see_nothing():
     for window in (0, 7, (1 << 31) - 1):
         for o in attend_both(st, 0.125, window=window):
             assert not bool(o[:2].any()) and not bool(o[3:].any()) and bool(o[2].any())
+
+
+@pytest.mark.parametrize("M,N,K,group", [(1, 300, 1024, 64), (5, 9000, 512, 128), (12, 300, 2080, 32), (1, 64, 32768, 256),
+                                         (20, 9000, 4096, 64)])
+@pytest.mark.parametrize("e", [-100, -90, 90, 100, 126])
+def test_w4_scales_to_the_ends_of_bf16(M, N, K, group, e):
+    """Scales and activations whose products stay in range, each near an end of its own."""
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
+    x, w, s, z = w4_case(M, N, K, group, True, BF, seed=35)
+    s = s.float().clamp(-0.9, 0.9)
+    s, x = (s * 2.0 ** e).to(BF), (x.float() * 2.0 ** max(-50, min(50, -e // 2))).to(BF)
+    assert bool(torch.isfinite(s).all())
+    w4_check(ops.gemv_w4(x.cuda(), w.cuda(), s.cuda(), z.cuda()), x, w, s, z)
