@@ -311,9 +311,11 @@ int dsv41_argmax_decode(const Dsv41ArgmaxArgs* a, void* stream);
  * rounded once to x's type: w unsigned 4-bit values packed two a byte, [N, K / 2] row-major (even
  * k in the low nibble) and read in place; scales [N, K / group] of x's type; zeros u8
  * [N, K / group] (values 0 .. 15) or 0 for 8 everywhere; x [M, x_ld] and y [M, y_ld] bf16 (below
- * 2^63 in magnitude), or f16 with f16 = 1. M <= 48, K a multiple of group, group a multiple of 32;
- * w and x 16-byte aligned, x_ld a multiple of 8. An infinity or NaN in a row of x makes that row of
- * y not finite, one in a scale that column. Up to 8 rows, and N K below 2^25, need no
+ * 2^63 in magnitude), or f16 with f16 = 1. The zero point may come off the sums, so a sum's fp32
+ * error is in proportion to sum |x| (w + z) |s| (weights that all equal z give about 0, not always 0),
+ * and bf16 terms are held to an absolute 2^-80 |s|. M <= 48, K a multiple of group, group a multiple
+ * of 32; w and x 16-byte aligned, x_ld a multiple of 8. An infinity or NaN in a row of x makes that
+ * row of y not finite, one in a scale that column. Up to 8 rows, and N K below 2^25, need no
  * scratch. No counterpart in the reference (its dense projections are FP8). */
 typedef struct {
   int64_t w, scales, zeros, x, y;     /* device pointers */

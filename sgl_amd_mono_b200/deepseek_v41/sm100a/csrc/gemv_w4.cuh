@@ -5,10 +5,12 @@
 // everything else rides along. What bounds the kernel beside them is the logic pipe that takes them
 // apart, so a nibble n goes into the tensor core as it stands: alone in the low mantissa bits it is
 // the subnormal n 2^-24 of f16 (n 2^-133 of bf16), exact like every product of m16n8k16 with x (bf16 x
-// is staged times 2^64, so that products stay in fp32's normal range). Zero points come off the fp32
-// sums: sum x (n - z) = sum x n - z sum x, the last sum taken once with the rows of x in shared memory
-// (where they do not fit, by the same instruction from a fragment of ones); it costs the sums an error of
-// at most 16 / |n - z| of their own.
+// is staged times 2^64, so that products stay in fp32's normal range down to x = 2^-57; smaller ones keep
+// an absolute 2^-80). Zero points come off the fp32 sums: sum x (n - z) = sum x n - z sum x, the last sum
+// taken once with the rows of x in shared memory (where they do not fit, by the same instruction from a
+// fragment of ones). So what the additions lose goes by sum |x| (n + z), not by sum |x (n - z)|: for weights
+// spread over 0 .. 15 about four times as much, and a group whose weights all equal its zero point leaves
+// that instead of exactly 0. Taking z off before the product costs a fourth of the logic instructions.
 // Weight rows are the mma's M, the rows of x its N. One word of a lane holds 8 consecutive k of a row;
 // masking word >> 4 i gives the pair (k_i, k_(i + 4)), and x is paired up the same way, so no nibble is
 // moved for order's sake: 7 logic instructions for 8 weights.

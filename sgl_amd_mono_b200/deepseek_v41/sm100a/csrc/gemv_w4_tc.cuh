@@ -16,7 +16,8 @@
 //
 // 48 rows of 129280 x 4096, groups of 64: 142 us, 2.1 TB/s of the weights and scales that bound it in
 // principle (46 us). The hand-over bounds it now: two converter warps a scheduler each convert, wait for the
-// MMA and read back in turn (logic pipe 44 %, tensor pipe 18 %, DRAM 26 %). Roundings: none but y's.
+// MMA and read back in turn (logic pipe 44 %, tensor pipe 18 %, DRAM 26 %). Weights, x and their
+// products are exact; the fp32 sums and y are rounded.
 #pragma once
 
 #include "gemv_w4.cuh"

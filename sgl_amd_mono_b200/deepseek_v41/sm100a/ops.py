@@ -37,7 +37,8 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch
             out: torch.Tensor | None = None) -> torch.Tensor:
     """[M, N] of x's type = x (bf16 or f16 [M, K], M <= 48) . dequant(w)^T, with w 4-bit values
     [N, K / 2] (even k in the low nibble), read in place, minus ``zeros`` (u8 [N, K / group]; 8
-    without them), times ``scales`` ([N, K / group] of x's type); group a multiple of 32."""
+    without them), times ``scales`` ([N, K / group] of x's type); group a multiple of 32. fp32 sums
+    whose error goes by sum |x| (w + zero) |scale|; bf16 x below 2^63 in magnitude."""
     if x.dim() != 2 or w.dim() != 2 or scales.dim() != 2:
         raise RuntimeError(f"gemv_w4: x {tuple(x.shape)}, w {tuple(w.shape)}, scales {tuple(scales.shape)}: want matrices")
     dev, dtype = x.get_device(), x.dtype

@@ -107,3 +107,43 @@ def test_w4_scales_to_the_ends_of_bf16(M, N, K, group, e):
     s, x = (s * 2.0 ** e).to(BF), (x.float() * 2.0 ** max(-50, min(50, -e // 2))).to(BF)
     assert bool(torch.isfinite(s).all())
     w4_check(ops.gemv_w4(x.cuda(), w.cuda(), s.cuda(), z.cuda()), x, w, s, z)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("M,N,K,group", [(1, 300, 1024, 128), (5, 333, 416, 32), (13, 2311, 4000, 32), (48, 2311, 1056, 96),
+                                         (20, 9000, 4096, 64)])
+def test_w4_weights_at_their_zero_point(M, N, K, group, dt):
+    """Rows and groups whose weights all equal the zero point: their terms are 0 within the contract's
+    bound, sum |x| (n + z) |s| times the additions' steps."""
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
+    x, w, s, z = w4_case(M, N, K, group, True, dt, seed=38)
+    z2 = z[:, :, None].expand(-1, -1, group // 2).reshape(N, -1)
+    at = (z2 | z2 << 4).to(torch.uint8)
+    w[::3] = at[::3]
+    w[1::3, :group // 2] = at[1::3, :group // 2]
+    y = ops.gemv_w4(x.cuda(), w.cuda(), s.cuda(), z.cuda()).cpu().double()
+    wd = G.w4_dequant(w, s, z)
+    ref = x.double() @ wd.T
+    assert bool((ref[:, ::3] == 0).all())
+    n = torch.stack([w & 15, w >> 4], -1).reshape(N, -1, group).double()
+    size = x.double().abs() @ ((n + z.double()[:, :, None]) * s.double().abs()[:, :, None]).reshape(N, -1).T
+    tol = half_step(dt) * ref.abs() + (K / 8 + 32) * 2.0 ** -23 * size + (2.0 ** -25 if dt == HF else 0)
+    off = ((y - ref).abs() / tol.clamp_min(1e-300)).max().item()
+    assert off <= 1, off
+
+
+@pytest.mark.parametrize("M,N,K,group", [(1, 300, 1024, 64), (12, 300, 2080, 32), (20, 9000, 4096, 64)])
+@pytest.mark.parametrize("e", [-50, -64, -80])
+def test_w4_small_activations(M, N, K, group, e):
+    """Activations of 2^-50 and less: the sums keep an absolute 2^-80 a term (the smallest fp32 number,
+    2^-149, times the 2^69 by which bf16 nibbles and activations are scaled)."""
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
+    x, w, s, z = w4_case(M, N, K, group, True, BF, seed=39)
+    x = (x.float() * 2.0 ** e).to(BF)
+    y = ops.gemv_w4(x.cuda(), w.cuda(), s.cuda(), z.cuda()).cpu().double()
+    wd = G.w4_dequant(w, s, z)
+    ref, size = x.double() @ wd.T, x.double().abs() @ wd.abs().T
+    zs = s.double().abs().sum(1) * group
+    tol = half_step(BF) * ref.abs() + (K / 8 + 32) * 2.0 ** -23 * size + 17 * 2.0 ** -80 * zs
+    off = ((y - ref).abs() / tol).max().item()
+    assert off <= 1, off
