@@ -35,7 +35,7 @@ def gemv_fp8(x: torch.Tensor, w: torch.Tensor, codes: torch.Tensor, x_group_rows
 
 def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None,
             out: torch.Tensor | None = None) -> torch.Tensor:
-    """[M, N] of x's type = x (bf16 or f16 [M, K], M <= 48) . dequant(w)^T, with w 4-bit values
+    """[M, N] of x's type = x (bf16 or f16 [M, K], M from 0 to 48) . dequant(w)^T, with w 4-bit values
     [N, K / 2] (even k in the low nibble), read in place, minus ``zeros`` (u8 [N, K / group]; 8
     without them), times ``scales`` ([N, K / group] of x's type); group a multiple of 32. fp32 sums
     whose error goes by sum |x| (w + zero) |scale|; bf16 x below 2^63 in magnitude."""
@@ -46,7 +46,7 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch
     (M, K), (N, groups), x_at, w_at = x.shape, scales.shape, x.data_ptr(), w.data_ptr()
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise RuntimeError(f"gemv_w4: x of {dtype}, want bfloat16 or float16")
-    if not 1 <= M <= W4_MAX_ROWS or not N or not groups or K % groups or K // groups % 32:
+    if M > W4_MAX_ROWS or not N or not groups or K % groups or K // groups % 32:
         raise RuntimeError(f"gemv_w4: {M} rows of {K} in {groups} groups, {N} outputs: at most {W4_MAX_ROWS} rows, groups "
                            "a multiple of 32")
     if w.shape != (N, K // 2) or w.dtype is not torch.uint8 or w.get_device() != dev or not w.is_contiguous() or w_at & 15:
@@ -77,6 +77,8 @@ def gemv_w4(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, zeros: torch
             raise RuntimeError(f"gemv_w4: out {tuple(out.shape)} {out.dtype} on {out.device} of strides {out.stride()}: "
                                f"want [{M}, {N}] {dtype} on {x.device}, contiguous rows")
         a.y_ld = y_ld
+    if not M:
+        return out
     a.y = out.data_ptr()
     if M > 8 and N * K >= 1 << 25:  # fewer rows and smaller matrices need no scratch
         need = ext.query("dsv41_gemv_w4_scratch_bytes", a)

@@ -147,3 +147,17 @@ def test_w4_small_activations(M, N, K, group, e):
     tol = half_step(BF) * ref.abs() + (K / 8 + 32) * 2.0 ** -23 * size + 17 * 2.0 ** -80 * zs
     off = ((y - ref).abs() / tol).max().item()
     assert off <= 1, off
+
+
+def test_w4_takes_an_empty_step():
+    """No rows give an empty output, as the cache's two operators take them."""
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
+    x, w, s, z = (t.cuda() for t in w4_case(3, 64, 256, 64, True, BF))
+    y = ops.gemv_w4(x[:0], w, s, z)
+    assert y.shape == (0, 64) and y.dtype == BF and y.is_cuda
+    out = torch.empty(0, 64, dtype=BF, device="cuda")
+    assert ops.gemv_w4(x[:0], w, s, z, out=out) is out
+    for bad in (dict(w=w[:50]), dict(scales=s.half()), dict(zeros=z.int()), dict(out=torch.empty(3, 64, dtype=BF, device="cuda")),
+                dict(x=x[:0].float())):
+        with pytest.raises(RuntimeError):
+            ops.gemv_w4(**{**dict(x=x[:0], w=w, scales=s, zeros=z), **bad})
