@@ -146,7 +146,7 @@ int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
   // else through 16, so that a prompt's warps nearly all find one block. A thread takes one query head
   // while the rows are too few to fill the GPU, else four, for which it reads the angles once.
   k.window = a->T >= 8 * a->seqs ? 16 : 1;
-  k.head_step = a->T * a->heads * a->dim / 16 < 148 * 2048 ? 1 : 4;
+  k.head_step = a->T * a->heads * a->dim / 16 < (int64_t)device_sms() * 2048 ? 1 : 4;
   const int64_t warps = cdiv64(a->T, k.window) * 2 * a->kv_heads;
   const int64_t q_threads = a->q ? a->T * cdiv64(a->heads, k.head_step) * (a->dim / 16) : 0;
   const int64_t kv_ctas = cdiv64(warps, kApThreads / 32), ctas = kv_ctas + cdiv64(q_threads, kApThreads);

@@ -161,3 +161,27 @@ def test_w4_takes_an_empty_step():
                 dict(x=x[:0].float())):
         with pytest.raises(RuntimeError):
             ops.gemv_w4(**{**dict(x=x[:0], w=w, scales=s, zeros=z), **bad})
+
+
+@pytest.mark.parametrize("neox,in_place", [(False, True), (True, False)])
+def test_append_prompts_take_four_heads_a_thread(neox, in_place):
+    """Enough rows that a thread rotates four query heads, the last one of ten two; a sequence without
+    rows and rows behind the last sequence."""
+    rows = [1500, 0, 1701, 1, 700]
+    st = Step(rows, [1500, 5, 1800, 40, 733], 10, 2, 128, 64, 16, BF, seed=36, tail=3)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert (sum(rows) + 3) * 10 * 128 // 16 >= sms * 2048
+    kv, qkv = st.cache(), st.qkv.cuda()
+    q, k, v = st.split(qkv)
+    cs = rope_table(1800, 128)
+    got = kv.append(k, v, q=q, cos_sin=cs.cuda(), neox=neox, q_out=q if in_place else None, **st.where())
+    qc, kc, vc = st.split(st.qkv)
+    G.append(st.k, st.kc, kc, st.cu, st.lens, st.table, cs, neox)
+    G.append(st.v, st.vc, vc, st.cu, st.lens, st.table)
+    assert torch.equal(kv.k_codes.cpu(), st.kc) and torch.equal(kv.v_codes.cpu(), st.vc)
+    assert same_bytes(kv.k, st.k) and same_bytes(kv.v, st.v)
+    used = sum(rows)
+    want = G.rotate_rows(qc, st.cu, st.lens, cs, neox, torch.zeros(qc.shape, dtype=BF))
+    assert torch.equal(got[:used].cpu(), want[:used])
+    if in_place:
+        assert torch.equal(qkv[used:].cpu(), st.qkv[used:]) and torch.equal(qkv[:, 10 * 128:].cpu(), st.qkv[:, 10 * 128:])
