@@ -218,9 +218,12 @@ struct PaShape {
   static_assert(kWarps / 2 * 8 * NT * D * 4 <= kRing, "the merge reuses the ring");
 };
 
-// What turns sum_i w_i V_i into the output: 2^(r - 7 - c) over the sum (0 where nothing was seen).
-__device__ __forceinline__ float pa_factor(float ref, float top, float sum) {
-  return sum == 0.f ? 0.f : ex2(ref - top - 7.f) / sum;
+// What turns sum_i w_i V_i into the output: 2^(r - 7 - c) over the sum (0 where nothing was seen), as two
+// factors, since the power alone may leave fp32's range (values' scales near either end of E8M0's) where
+// the output does not.
+__device__ __forceinline__ float2 pa_factor(float ref, float top, float sum) {
+  const float e = ref - top - 7.f, half = 0.5f * e;
+  return sum == 0.f ? make_float2(0.f, 0.f) : make_float2(ex2(half) / sum, ex2(e - half));
 }
 
 // out[8 dims] of one column from 8 consecutive values.
@@ -667,13 +670,13 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
           if (whole) {
             float sum = l[n][e];
             if (a.sink) sum += ex2(a.sink[h] * 1.44269504f - top[n][e]);
-            const float f = pa_factor(ref[n][e], top[n][e], sum);
+            const float2 f = pa_factor(ref[n][e], top[n][e], sum);
             T* y = reinterpret_cast<T*>(a.out) + (w.row0 + j) * a.out_ld + h * D;
 #pragma unroll
             for (int i = 0; i < KS / 4; ++i) {
               float x[8];
 #pragma unroll
-              for (int b = 0; b < 8; ++b) x[b] = o[n][4 * i + b / 2][e + 2 * (b & 1)] * f;
+              for (int b = 0; b < 8; ++b) x[b] = o[n][4 * i + b / 2][e + 2 * (b & 1)] * f.x * f.y;
               *reinterpret_cast<uint4*>(y + (i / 2) * 128 + d0 + (i & 1) * 8) = pack8<F16>(x);
             }
           } else {
@@ -744,9 +747,10 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const PagedA
   for (int w = 0; w < kPaJoinThreads / 32; ++w) sum += red[2][w];
   const int col = sp.col0 + c, group = a.heads / a.cache.kv_heads, h = sp.h0 + col % group;
   if (a.sink) sum += ex2(a.sink[h] * 1.44269504f - top);
-  const float f = pa_factor(m, top, sum);
+  const float2 f = pa_factor(m, top, sum);
   T* y = reinterpret_cast<T*>(a.out) + (int64_t)(sp.row0 + col / group) * a.out_ld + h * D + 4 * d;
-  *reinterpret_cast<uint2*>(y) = make_uint2(Act<F16>::pack(o.x * f, o.y * f), Act<F16>::pack(o.z * f, o.w * f));
+  *reinterpret_cast<uint2*>(y) = make_uint2(Act<F16>::pack(o.x * f.x * f.y, o.y * f.x * f.y),
+                                            Act<F16>::pack(o.z * f.x * f.y, o.w * f.x * f.y));
 }
 
 }  // namespace dsv41

@@ -185,3 +185,15 @@ def test_append_prompts_take_four_heads_a_thread(neox, in_place):
     assert torch.equal(got[:used].cpu(), want[:used])
     if in_place:
         assert torch.equal(qkv[used:].cpu(), st.qkv[used:]) and torch.equal(qkv[:, 10 * 128:].cpu(), st.qkv[:, 10 * 128:])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("code", [0, 1, 4, 8, 12])
+def test_attend_small_values_everywhere(code, dim):
+    """Every value under a scale near the smallest that E8M0 holds: bf16 outputs hold them still."""
+    st = Step([1, 1], [300, 21], 2, 1, dim, 16, 16, BF, seed=37)
+    st.vc.fill_(code)
+    ref, sizes = G.attend(st.split(st.qkv)[0], st.k, st.v, st.kc, st.vc, st.cu, st.lens, st.table, 0.125)
+    for o in attend_both(st, 0.125):
+        # (and half a step of bf16 below its smallest normal number)
+        assert bool(((o.double() - ref).abs() <= attn_tol(BF, ref, sizes) + 2.0 ** -134).all())
