@@ -121,6 +121,12 @@ __device__ __forceinline__ bool wt_wait(uint32_t bar, uint32_t parity, volatile 
   atomicExch(&g_tc_error, 1);
   return false;
 }
+// Wait for what is in flight into this CTA's memory, after an abort too (bounded like the others).
+__device__ __forceinline__ void wt_land(uint32_t bar, uint32_t parity) {
+  const uint64_t deadline = wt_now() + 2000000000ull;
+  while (!wt_try(bar, parity) && wt_now() < deadline) {
+  }
+}
 
 template <bool F16, int NP, int SUB>
 __global__ void __launch_bounds__(kWtThreads, 1)
@@ -186,10 +192,8 @@ __global__ void __launch_bounds__(kWtThreads, 1)
             : "memory");
         if (++kb == p.kblocks) kb = 0, ++tile;
       }
-      // copies still in flight land before the CTA can exit (bounded, also after an abort)
-      for (int k = max(0, i - SW); k < i; ++k)
-        for (uint32_t it = 0; it < kTcWaitPolls && !mbar_try(w_full(k % SW), (k / SW) & 1); ++it) {
-        }
+      // copies still in flight land before the CTA can exit
+      for (int k = max(0, i - SW); k < i; ++k) wt_land(w_full(k % SW), (k / SW) & 1);
     }
   } else if (warp == 1 || warp == 6) {
     if (lane == 0) {
@@ -218,8 +222,9 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         umma_commit(x_empty(xs));
         if (++kb == p.kblocks) kb = 0;
       }
+      // and MMAs read and write TMEM before it is freed
       umma_commit(drained(h));
-      wt_wait(drained(h), 0, abort);
+      wt_land(drained(h), 0);
     }
   } else if (warp >= 2 && warp < 6) {
     const int et = tid - 64;
