@@ -195,6 +195,10 @@ class PagedKV:
         if not 0 <= window < 1 << 31:
             raise RuntimeError(f"window {window}")
         a.window = window
+        try:
+            a.scale_f32 = _U32.unpack(_F32.pack(scale))[0]
+        except (OverflowError, struct.error):
+            raise RuntimeError(f"scale {scale}: want a number in fp32's range") from None
         if sink is not None:
             if sink.shape != (heads,) or sink.dtype is not torch.float32 or sink.get_device() != self._dev \
                     or not sink.is_contiguous():
@@ -202,7 +206,6 @@ class PagedKV:
             a.sink = sink.data_ptr()
         if not rows or not a.seqs:
             return out
-        a.scale_f32 = _U32.unpack(_F32.pack(scale))[0]
         need = ext.query("dsv41_paged_attn_scratch_bytes", a)
         if need:
             scratch = self.k.new_empty((need,))

@@ -197,3 +197,14 @@ def test_attend_small_values_everywhere(code, dim):
     for o in attend_both(st, 0.125):
         # (and half a step of bf16 below its smallest normal number)
         assert bool(((o.double() - ref).abs() <= attn_tol(BF, ref, sizes) + 2.0 ** -134).all())
+
+
+def test_scales_that_fp32_does_not_hold_are_refused():
+    st = Step([1], [20], 4, 2, 64, 16, 16, BF, seed=46, cu=False)
+    kv, w = st.cache(), st.where()
+    q = st.split(st.qkv.cuda())[0]
+    for scale in (1e39, -1e300, "1", None):
+        for x, where in ((q, w), (q[:0], dict(lens=w["lens"][:0], table=w["table"][:0]))):
+            with pytest.raises(RuntimeError, match="scale"):
+                kv.attend(x, scale=scale, **where)
+    assert torch.equal(kv.attend(q, scale=0.125, **w), kv.attend(q, scale=torch.tensor(0.125), **w))
