@@ -208,3 +208,54 @@ def test_scales_that_fp32_does_not_hold_are_refused():
             with pytest.raises(RuntimeError, match="scale"):
                 kv.attend(x, scale=scale, **where)
     assert torch.equal(kv.attend(q, scale=0.125, **w), kv.attend(q, scale=torch.tensor(0.125), **w))
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("dim,group", INSTANCES)
+def test_attend_every_instance_whole_and_split(dim, group, dt):
+    st = Step([1, 1, 1, 1], [777, 0, 131, 16], group * 2, 2, dim, 32, 16, dt, seed=41)
+    sink = torch.randn(st.heads, generator=st.g)
+    for window, sk in ((0, None), (200, sink)):
+        ref, sizes = G.attend(st.split(st.qkv)[0], st.k, st.v, st.kc, st.vc, st.cu, st.lens, st.table, dim ** -0.5, window, sk)
+        for o in attend_both(st, dim ** -0.5, window, sk):
+            assert bool(((o.double() - ref).abs() <= attn_tol(dt, ref, sizes)).all())
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("rows,heads,kvh", [([6, 6, 6], 8, 2), ([3, 0, 9], 8, 2), ([5, 5], 12, 4), ([2, 7, 3], 6, 1)])
+def test_attend_verify_rows_split(rows, heads, kvh, dt):
+    """Rows of several tokens over 9 to 32 columns, whole and split."""
+    st = Step(rows, [500, 77, 260][:len(rows)], heads, kvh, 128, 32, 16, dt, seed=42)
+    ref, sizes = G.attend(st.split(st.qkv)[0], st.k, st.v, st.kc, st.vc, st.cu, st.lens, st.table, 0.1)
+    for o in attend_both(st, 0.1):
+        assert bool(((o.double() - ref).abs() <= attn_tol(dt, ref, sizes)).all())
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("M,N,K,group", [
+    (48, 8200, 4096, 128), (33, 9000, 4096, 256), (32, 8200, 4096, 32), (17, 8300, 4224, 32), (1, 8192, 4096, 32),
+    (8, 300, 8192, 32), (2, 5000, 16384, 128), (3, 200, 16384, 256), (4, 130, 32768, 64), (16, 200, 16384, 128)])
+def test_w4_every_instance(M, N, K, group, zeros, dt):
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
+    x, w, s, z = (None if t is None else t.cuda() for t in w4_case(M, N, K, group, zeros, dt, seed=43))
+    w4_check(ops.gemv_w4(x, w, s, z), x, w, s, z)
+
+
+def test_w4_non_finite_stays_in_its_row_and_column_of_a_large_matrix():
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
+    x, w, s, z = w4_case(20, 9000, 4096, 64, True, BF, seed=44)
+    x[1, 100], x[7, 4000] = float("inf"), float("nan")
+    s[8999, 3] = float("nan")
+    y = ops.gemv_w4(x.cuda(), w.cuda(), s.cuda(), z.cuda()).cpu()
+    bad, want = ~torch.isfinite(y), torch.zeros(20, 9000, dtype=torch.bool)
+    want[1], want[7], want[:, 8999] = True, True, True
+    assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("neox", [False, True])
+@pytest.mark.parametrize("dim,rope", [(128, 128), (256, 256), (128, 64), (256, 16)])
+def test_append_rotates_whole_and_part_heads(dim, rope, neox, dt):
+    st = Step([3, 0, 20, 1], [40, 9, 77, 48], 6, 2, dim, 32, 16, dt, seed=45, tail=2)
+    run_append(st, rope=rope, neox=neox, in_place=not neox)
