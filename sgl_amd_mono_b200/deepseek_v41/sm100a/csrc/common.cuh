@@ -38,6 +38,20 @@ __device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t v) {
   return pack_f16x2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
+// 2^x by the SFU's ex2 instruction (PTX ex2.approx.ftz.f32: about 2 ulp; results below 2^-126
+// flush to 0, far under what the f16 head/tail of p can hold).
+__device__ __forceinline__ float ex2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// {lo, hi} -> f16x2 bits (round to nearest), one instruction.
+__device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // e4m3fn byte of x clamped to +-448 (round to nearest even).
 __device__ __forceinline__ uint8_t e4m3_byte(float x) {
   x = fminf(fmaxf(x, -kFp8Max), kFp8Max);

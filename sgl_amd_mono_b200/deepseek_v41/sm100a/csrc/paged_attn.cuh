@@ -167,11 +167,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 // f16x2 of the low and of the high two e4m3 bytes of w (exact, NaN kept).
 __device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }"
@@ -184,12 +179,6 @@ __device__ __forceinline__ void pa_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// {lo, hi} rounded to f16x2 by one instruction.
-__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
 }
 template <class V>
 __device__ __forceinline__ V pa_lds(const uint8_t* p) {
@@ -223,7 +212,7 @@ struct PaShape {
 // the output does not.
 __device__ __forceinline__ float2 pa_factor(float ref, float top, float sum) {
   const float e = ref - top - 7.f, half = 0.5f * e;
-  return sum == 0.f ? make_float2(0.f, 0.f) : make_float2(ex2(half) / sum, ex2(e - half));
+  return sum == 0.f ? make_float2(0.f, 0.f) : make_float2(ex2_approx(half) / sum, ex2_approx(e - half));
 }
 
 // out[8 dims] of one column from 8 consecutive values.
@@ -489,9 +478,9 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
             float m = fmaxf(s[n][e], s[n][e + 2]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            const float r = fmaxf(m + ev, ref[n][e]), f = ex2(ref[n][e] - r);
+            const float r = fmaxf(m + ev, ref[n][e]), f = ex2_approx(ref[n][e] - r);
             m = fmaxf(m, top[n][e]);
-            l[n][e] *= ex2(top[n][e] - m);
+            l[n][e] *= ex2_approx(top[n][e] - m);
             ref[n][e] = r;
             top[n][e] = m;
 #pragma unroll
@@ -502,16 +491,16 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) l[n][e] += ex2(s[n][e] - top[n][e]) + ex2(s[n][e + 2] - top[n][e]);
+        for (int e = 0; e < 2; ++e) l[n][e] += ex2_approx(s[n][e] - top[n][e]) + ex2_approx(s[n][e + 2] - top[n][e]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = ex2(s[n][e] + (ev + 7.f - ref[n][e & 1]));
+        for (int e = 0; e < 4; ++e) s[n][e] = ex2_approx(s[n][e] + (ev + 7.f - ref[n][e & 1]));
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float x = s[n][2 * e], y = s[n][2 * e + 1];
-          const uint32_t head = pa_pack(x, y);
+          const uint32_t head = cvt_f16x2(x, y);
           const float2 h = Act<true>::unpack(head);
           ph[n][e] = movmatrix(head);
-          pl[n][e] = movmatrix(pa_pack(x - h.x, y - h.y));
+          pl[n][e] = movmatrix(cvt_f16x2(x - h.x, y - h.y));
         }
       }
 
@@ -620,9 +609,9 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const float4 x = rl_sm[i * 8 * NT + 8 * n + 2 * t + e];
-          sum = fmaf(x.z, ex2(x.y - c), sum);
+          sum = fmaf(x.z, ex2_approx(x.y - c), sum);
         }
-        const float f = ex2(ref[n][e] - m);
+        const float f = ex2_approx(ref[n][e] - m);
 #pragma unroll
         for (int i = 0; i < KS; ++i) o[n][i][e] *= f, o[n][i][e + 2] *= f;
         ref[n][e] = m;
@@ -669,7 +658,7 @@ __global__ void __launch_bounds__(32 * PaShape<D, NT>::kWarps, PaShape<D, NT>::k
           const int d0 = D == 64 ? 8 * g : 16 * ((g >> 1) | (g & 1) << 2);
           if (whole) {
             float sum = l[n][e];
-            if (a.sink) sum += ex2(a.sink[h] * 1.44269504f - top[n][e]);
+            if (a.sink) sum += ex2_approx(a.sink[h] * 1.44269504f - top[n][e]);
             const float2 f = pa_factor(ref[n][e], top[n][e], sum);
             T* y = reinterpret_cast<T*>(a.out) + (w.row0 + j) * a.out_ld + h * D;
 #pragma unroll
@@ -722,7 +711,7 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const PagedA
   for (int w = 0; w < kPaJoinThreads / 32; ++w) m = fmaxf(m, red[0][w]), top = fmaxf(top, red[1][w]);
   for (int i = tid; i < sp.pieces; i += kPaJoinThreads) {
     const float4 rl = a.part_rl[at(i)];
-    sum = fmaf(rl.z, ex2(rl.y - top), sum);
+    sum = fmaf(rl.z, ex2_approx(rl.y - top), sum);
   }
   sum = warp_sum(sum);
   if (lane == 0) red[2][warp] = sum;
@@ -730,7 +719,7 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const PagedA
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int i = pg; i < sp.pieces; i += PG) {
-    const float f = ex2(a.part_rl[at(i)].x - m);
+    const float f = ex2_approx(a.part_rl[at(i)].x - m);
     const float4 y = *reinterpret_cast<const float4*>(a.part + at(i) * D + 4 * d);
     o.x = fmaf(y.x, f, o.x), o.y = fmaf(y.y, f, o.y), o.z = fmaf(y.z, f, o.z), o.w = fmaf(y.w, f, o.w);
   }
@@ -746,7 +735,7 @@ __global__ void __launch_bounds__(kPaJoinThreads) paged_join_kernel(const PagedA
 #pragma unroll
   for (int w = 0; w < kPaJoinThreads / 32; ++w) sum += red[2][w];
   const int col = sp.col0 + c, group = a.heads / a.cache.kv_heads, h = sp.h0 + col % group;
-  if (a.sink) sum += ex2(a.sink[h] * 1.44269504f - top);
+  if (a.sink) sum += ex2_approx(a.sink[h] * 1.44269504f - top);
   const float2 f = pa_factor(m, top, sum);
   T* y = reinterpret_cast<T*>(a.out) + (int64_t)(sp.row0 + col / group) * a.out_ld + h * D + 4 * d;
   *reinterpret_cast<uint2*>(y) = make_uint2(Act<F16>::pack(o.x * f.x * f.y, o.y * f.x * f.y),
