@@ -259,3 +259,68 @@ def test_w4_non_finite_stays_in_its_row_and_column_of_a_large_matrix():
 def test_append_rotates_whole_and_part_heads(dim, rope, neox, dt):
     st = Step([3, 0, 20, 1], [40, 9, 77, 48], 6, 2, dim, 32, 16, dt, seed=45, tail=2)
     run_append(st, rope=rope, neox=neox, in_place=not neox)
+
+
+@pytest.mark.parametrize("M,group,zeros,dt", [(1, 128, True, BF), (7, 64, False, HF), (20, 64, True, HF)])
+def test_w4_weights_past_four_gigabytes(M, group, zeros, dt):
+    """More weights than 32 bits of bytes: the last and the first rows against 64 bits."""
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
+    N, K = 530003, 16384
+    assert N * K // 2 > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(47)
+    w = torch.randint(0, 256, (N, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    s = (torch.rand(N, K // group, generator=g, device="cuda") * 0.02 + 1e-3).to(dt)
+    z = torch.randint(0, 16, (N, K // group), generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+    x = torch.randn(M, K, generator=g, device="cuda").to(dt)
+    y = ops.gemv_w4(x, w, s, z)
+    for part in (slice(0, 600), slice(N // 2, N // 2 + 300), slice(N - 600, N)):
+        w4_check(y[:, part], x, w[part], s[part], None if z is None else z[part])
+
+
+def test_append_positions_past_the_angles_read_the_last_row():
+    st = Step([3, 0, 20, 1], [40, 9, 77, 48], 6, 2, 128, 32, 16, BF, seed=48)
+    cs = rope_table(45, 128)
+    kv, w = st.cache(), st.where()
+    q, k, v = st.split(st.qkv.cuda())
+    got = kv.append(k, v, q=q, cos_sin=cs.cuda(), neox=True, **w)
+    qc, kc, vc = st.split(st.qkv)
+    G.append(st.k, st.kc, kc, st.cu, st.lens, st.table, cs, True)
+    assert torch.equal(kv.k_codes.cpu(), st.kc) and same_bytes(kv.k, st.k)
+    assert torch.equal(got.cpu(), G.rotate_rows(qc, st.cu, st.lens, cs, True, torch.zeros(qc.shape, dtype=BF)))
+
+
+def test_calls_of_two_streams_and_two_graphs_at_once():
+    """The large products, whose scratch and TMEM are a call's own, and the split attention: eager on two
+    streams together, then two captured graphs replayed together."""
+    from sgl_amd_mono_b200.deepseek_v41.sm100a import ops
+    st = Step([1, 1], [3000, 70], 16, 2, 128, 32, 16, BF, seed=49)
+    kv, where = st.cache(), st.where()
+    q = st.split(st.qkv.cuda())[0]
+    cases = [tuple(t.cuda() for t in w4_case(20, 9000, 4096, 64, True, BF, seed=s)) for s in (50, 51)]
+
+    def calls(i):
+        return ops.gemv_w4(*cases[i]), kv.attend(q, scale=0.05 * (i + 1), **where), ops.gemv_w4(*cases[1 - i])
+
+    ref = [calls(0), calls(1)]
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, s in enumerate(side):
+            with torch.cuda.stream(s):
+                got[i].append(calls(i))
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in side]
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g, stream=side[i]):
+            got[i].append(calls(i))
+    for _ in range(10):
+        for g, s in zip(graphs, side):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for r, outs in zip(ref, got):
+        for o in outs:
+            assert all(torch.equal(a, b) for a, b in zip(r, o))
+    from sgl_amd_mono_b200.common import ext
+    assert ext.lib().dsv41_device_error() == 0
