@@ -347,7 +347,8 @@ int dsv41_gemv_w4(const Dsv41GemvW4Args* a, void* stream);
  * have; when it grows, the older tokens' bytes are rounded again to the new scale. Values are
  * rounded to nearest even and saturate at 448 c; an infinity counts as the largest float, NaN stays
  * NaN and moves no scale. Tokens whose page is out of range (table entry outside [0, pages), or a
- * position outside [0, width * page)) are skipped. No counterpart in the reference (its records
+ * position outside [0, width * page)) are skipped. T kv_heads up to about 2^26 (2^30 with 8 rows a sequence
+ * and more) and T heads dim up to about 2^38. No counterpart in the reference (its records
  * hold one shared latent a token with a scale per token, front.py:246-300). */
 typedef struct {
   int64_t T, seqs, heads, kv_heads, dim, rope, neox, f16;

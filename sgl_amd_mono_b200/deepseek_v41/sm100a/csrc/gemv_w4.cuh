@@ -19,7 +19,8 @@
 // warp streams its chunks through a ring of its own by 16-byte cp.async, across row tiles without a
 // pause. The warps' sums meet in shared memory in warp order, so the result does not depend on timing.
 //
-// One row: 1024 x 1024 2.3 us (launch and one latency), 8192 x 4096 6.6 us (2.7 TB/s: two tiles a CTA),
+// One row: 1024 x 1024 2.3 us (launch and one latency), 8192 x 4096 6.5 us (2.7 TB/s: a tile a CTA and two
+// chunks a warp, of which the second waits until x is staged),
 // 65536 x 8192 at 4.3 TB/s, where the logic pipe issues 63 % of what it can and DRAM is at 53 %.
 #pragma once
 

@@ -88,12 +88,16 @@ int64_t attn_go(const Dsv41PagedAttnArgs* a, F f) {
 // steps of an item, the rows the items. Whole items, a CTA each, take one launch and no scratch; or the
 // GPU's CTAs share all steps, no more of them than there can be, and a second launch joins the pieces.
 // Whole, the CTAs without an item idle for up to steps (1 - items / fit); split, each CTA starts and ends
-// two pieces or so. Whole against split, us of GPU time, heads of 128, groups of 8: 4 items of 3 steps 7.7
-// and 8.7, 7 steps 10.1 and 9.3 (but 10.8 and 15.7 a call); 64 items of 11 steps 13.8 and 17.6, 16 steps
-// 16.9 and 14.7; 256 of 8 steps 15.2 and 23.7; 1024 of 4 steps 45.4 and 44.3, of uneven 4 steps 36.6 and
-// 57.1. With more columns or dim 256 a step costs more: 16 items of dim 256, 3 steps 14.4 and 14.9, 4 steps
-// 15.9 and 15.0; 72 of 32 columns, 8 steps 24.2 and 23.4, 16 steps 36.3 and 29.5. At most 16 steps, since
-// one long sequence may be the only one; at most four waves of CTAs, since each has to find its item.
+// two pieces or so. Whole against split, us of GPU time (and of a call from Python, where they differ much),
+// heads of 128, groups of 8: 4 items of 3 steps 8.1 and 8.8 (10.9 and 16.1), 7 steps 11.1 and 9.2 (11.7 and
+// 16.0); 64 items of 11 steps 14.3 and 18.3, 16 steps 18.3 and 15.9; 256 of 8 steps 19.8 and 28.2; 1024 of 4
+// steps 47.5 and 46.7, of uneven 4 steps 39.8 and 62.6. With more columns or dim 256 a step costs more: 16
+// items of dim 256, 3 steps 13.7 and 13.3, 4 steps 15.3 and 13.5; 72 of 32 columns, 8 steps 25.0 and 23.0, 16
+// steps 37.1 and 31.3. So the rule takes the faster form where there are many items, and the faster call
+// where there are few: a captured step loses 2 us there at most, an eager one would lose 5. It misses the
+// faster form near its border (64 items of 11 steps are split) and, since items counts what the rows could
+// fill at worst, in the last example. At most 16 steps, since one long sequence may be the only one; at most
+// four waves of CTAs, since each has to find its item.
 struct AttnPlan {
   int64_t ctas, scratch;
   bool whole;
@@ -150,7 +154,7 @@ int dsv41_kv_append(const Dsv41KvAppendArgs* a, void* stream) {
   const int64_t warps = cdiv64(a->T, k.window) * 2 * a->kv_heads;
   const int64_t q_threads = a->q ? a->T * cdiv64(a->heads, k.head_step) * (a->dim / 16) : 0;
   const int64_t kv_ctas = cdiv64(warps, kApThreads / 32), ctas = kv_ctas + cdiv64(q_threads, kApThreads);
-  if (ctas > UINT32_MAX / kApThreads) return DSV41_EINVAL;  // no memory holds as many rows
+  if (ctas > UINT32_MAX / kApThreads) return DSV41_EINVAL;  // threads are counted in 32 bits
   k.kv_ctas = (int)kv_ctas;
   const dim3 grid((unsigned)ctas), cta(kApThreads);
   auto by_pairs = [&](auto f16, auto d) {

@@ -11,9 +11,11 @@
 // half a rotation apart for (j, j + rope / 2). A block's rows are looked at twice, for the largest
 // magnitude and to be written, some of them in registers and the others from L1.
 //
-// One token 3.2 us and 8 sequences of 6 rows 3.6: dependent latencies (row, length, page, code). Prompts of
-// 10266 rows, 32 query and 8 kv heads of 128: 47 us (5.0 TB/s of 236 MB). The queries alone take 29 us, a copy of
-// them 27; the keys and values 23, which is latency and the second look, not bytes (10 us).
+// One token 3.1 us and 8 sequences of 6 rows 3.6: dependent latencies (row, length, page, code). Prompts of
+// 10266 rows, 32 query and 8 kv heads of 128: 48 us (4.9 TB/s of 236 MB). The queries alone take 29 us, a copy of
+// them 27; the keys and values 23, which is latency and the second look, not bytes (10 us). Four CTAs an SM leave
+// 64 registers a thread, of which every instance spills some (60 bytes reloaded with pairs side by side, 128
+// half a rotation apart); fewer CTAs were slower (59 us to 53 when that was measured).
 #pragma once
 
 #include "gqa.cuh"

@@ -21,7 +21,7 @@
 // keeps it to 2^-22 of itself and 2^-32 of the column's largest. The head alone (2^-11) showed: outputs
 // 8e-4 (bf16) and 3e-4 (f16) of their size away from those of fp32 weights, now 1e-4 or less but over
 // the longest contexts. The tails' product costs 2 % with one column tile (95 to 97 us for 48 rows at
-// 8192 tokens, 182 to 187 for 4 at 131072) and 13 % with three (147 to 167).
+// 8192 tokens, 182 to 186 for 4 at 131072) and 13 % with three (147 to 167).
 //
 // Split. The work (sequence, kv head, column tile, steps of 16 W tokens) is cut into equal
 // contiguous shares, one a CTA, whatever the lengths: each CTA finds its own from the lengths on the
@@ -29,7 +29,7 @@
 // joins the pieces in order, so the sums do not depend on timing. Where pages or window keep
 // the items short, and there are not a few items only, they are not split and one launch does.
 //
-// 4 rows of 64 heads over 131072 tokens, 8 kv heads: 187 us, its bytes take 0.88 of that. With up to 16
+// 4 rows of 64 heads over 131072 tokens, 8 kv heads: 186 us, its bytes take 0.88 of that. With up to 16
 // columns DRAM bounds it; with more, latencies between the dependent products and conversions of a tile
 // on the two or three warps a scheduler that their registers leave (8 x 6 rows, 24 columns, at 32768
 // tokens: 167 us for 82 us of bytes), some of which spill (24 columns of 128 dims: 255 registers, 232
@@ -190,8 +190,9 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w &
 template <int D, int NT>
 struct PaShape {
   // What a thread holds decides how many warps an SM runs: two CTAs of 8 while O takes up to 32 registers
-  // (and the fragments of Q as many), one of 12 up to 64, else one of 8 (8 sequences at 32768 tokens: O of
-  // 64 121 us with 12 warps, 125 with two CTAs of 8, 140 with 8; O of 96 192 us with 12 and 154 with 8).
+  // (and the fragments of Q as many), one of 12 up to 64, else one of 8 (8 sequences at 32768 tokens, dim
+  // 128: O of 64 123 us with 12 warps, 128 with two CTAs of 8, 126 with 8; O of 96 179 us with 12 and 171 with 8;
+  // dim 256 at 16384 tokens, O of 64: 104, 108 and 99).
   static constexpr int kO = NT * D / 4;               // O registers a thread
   static constexpr int kCtas = kO <= 32 ? 2 : 1;      // an SM
   static constexpr int kWarps = kO <= 32 || kO > 64 ? 8 : 12;

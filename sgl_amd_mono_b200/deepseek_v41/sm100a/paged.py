@@ -140,7 +140,8 @@ class PagedKV:
         [positions, rope] fp32 (rope / 2 cos, then rope / 2 sin) the last ``rope`` dims of the keys,
         and of the queries ``q`` [T, heads, dim] where given, are rotated by their positions, in
         pairs (2j, 2j + 1) or, ``neox``, (j, j + rope / 2). Returns the rotated queries (``q_out``,
-        which may be ``q``, or a new tensor), or None without ``q``. A sequence's pages must not be
+        which may be ``q``, or a new tensor), or None without ``q``; rows behind the last sequence are
+        left as they were (unset in a new tensor). A sequence's pages must not be
         another's: two sequences that append to one block race."""
         stream = current_stream(self._dev, "PagedKV.append")
         a = abi.KvAppendArgs.from_buffer_copy(self._append_args)
@@ -180,7 +181,7 @@ class PagedKV:
         rows), with ``window`` the last ``window`` of them; ``scale`` times q . k goes into the
         softmax, with ``sink`` [heads] fp32 as one more score without a value. A row that sees
         nothing gives zeros. Returns ``out`` (or a new tensor) [T, heads, dim]; rows behind the last
-        sequence are left as they were."""
+        sequence are left as they were (unset in a new tensor)."""
         stream = current_stream(self._dev, "PagedKV.attend")
         a = abi.PagedAttnArgs.from_buffer_copy(self._attend_args)
         rows, dtype = self._step(a, q, "q", lens, table, cu_rows)
