@@ -19,8 +19,8 @@
 // (exact but for values 2^-29 below the column's largest). Scores, weights, sums and O are fp32. A
 // weight enters the second product as two f16 numbers, its head and what the head leaves, which
 // keeps it to 2^-22 of itself and 2^-32 of the column's largest. The head alone (2^-11) showed: outputs
-// 8e-4 (bf16) and 3e-4 (f16) of their size away from those of fp32 weights, now 5e-5 or less (bf16, 131072
-// tokens: 1.7e-4). The tails' product costs 2 % with one column tile (95 to 97 us for 48 rows at 8192
+// 8e-4 (bf16) and 3e-4 (f16) of their size away from those of fp32 weights, now 1e-4 or less (bf16, 131072
+// tokens: up to 1.7e-4). The tails' product costs 2 % with one column tile (95 to 97 us for 48 rows at 8192
 // tokens, 182 to 186 for 4 at 131072) and 13 % with three (147 to 167). What is left over long contexts is
 // the tensor core's truncation of its fp32 sums, up to 2^-23 of O a product: each tile's product by
 // itself and added to O with rounding has 2e-5 at 131072 tokens, but costs 9 to 11 % (spills; 108 us, 203
